@@ -33,6 +33,7 @@
 //   attn_prefill_kernel  sequences with more rows: 128-row workgroups share
 //                        K/V tiles dequantized to fp16 in LDS; 32x32x16 MFMA
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <mutex>
 #include <type_traits>
@@ -148,7 +149,41 @@ struct AttnParams {
     const void *new_k, *new_v;
     int64_t nk_ts, nk_hs, nv_ts, nv_hs;  // element strides
     const int64_t *new_slot;
+    // Scored attention (the kernels' SC parameter, not SC_NONE).  SC_CAP:
+    // cap_log2e = cap * log2 e, and scale_log2e (and with it pf_qmul * pf_kmul)
+    // is 2 * log2 e * scale / cap.  SC_BIAS: one slope per query head.  tree
+    // (SC_TREE; SC_CAP where given): a 64-bit mask per query row.
+    float cap_log2e;
+    const float *slopes;
+    const int64_t *tree;
 };
+
+// Score forms of the attention kernels.  With s = scale * q.k:
+//   SC_NONE  s
+//   SC_TREE  s; the sequence's last n_q keys are the nodes of a tree, and row j
+//            sees every key before them and the nodes i <= j of bit i in its mask
+//   SC_CAP   cap * tanh(s / cap), over causal rows or a tree's
+//   SC_BIAS  s + slope[head] * (key position - row position)
+constexpr int SC_NONE = 0, SC_TREE = 1, SC_CAP = 2, SC_BIAS = 3;
+
+// cap * tanh(s / cap) in log2 units, from x = 2 log2 e * s / cap: with t = 2^x,
+// tanh = 1 - 2 / (1 + t), exact at both ends (t = 0, inf) and within 2e-7 * cap
+// of it between.  less: subtracted from the result (a running max).
+__device__ __forceinline__ float capped(float x, float cap_log2e, float less) {
+    return fmaf(-2.0f * cap_log2e, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), cap_log2e - less);
+}
+
+// Whether a row with tree mask m sees node `node` (keys before the tree have
+// a negative one).
+__device__ __forceinline__ bool tree_sees(uint64_t m, int node) {
+    return (uint32_t)node < 64u && ((m >> (node & 63)) & 1u);
+}
+
+// A row's mask without the nodes after its own (row j is node j).
+__device__ __forceinline__ uint64_t tree_row(const AttnParams &p, int q0, int j) {
+    const uint64_t m = (uint64_t)p.tree[q0 + j];
+    return j >= 63 ? m : m & ((2ull << j) - 1);
+}
 
 __device__ __forceinline__ int seq_q0(const AttnParams &p, int s) { return p.qsl ? p.qsl[s] : s * p.uq_rows; }
 __device__ __forceinline__ int seq_nq(const AttnParams &p, int s) { return p.qsl ? p.qsl[s + 1] - p.qsl[s] : p.uq; }
@@ -376,6 +411,136 @@ __device__ __forceinline__ void attend_subpage(WaveAcc<NRG> &acc, const SubPage 
     }
 }
 
+// fp16 pair with Inf / NaN replaced by +-65504 (v_pk_max/min_f16 return the
+// non-NaN operand).
+__device__ __forceinline__ half2_t finite2(half2_t x) {
+    const half2_t hi = {(half_t)65504.0f, (half_t)65504.0f};
+    return __builtin_elementwise_min(__builtin_elementwise_max(x, -hi), hi);
+}
+
+// What the scored forms hold for a lane's rows (row group rg: row row0 + 16 rg
+// + i16).
+template <int NRG, int SC>
+struct ScoreRows {
+    float cap;                // SC_CAP: cap * log2 e
+    float slope[NRG];         // SC_BIAS: slope * log2 e
+    int pos[NRG];             //          the row's position
+    uint64_t tree[NRG];       // SC_TREE, SC_CAP: the nodes the row sees,
+    int node0;                //                  and the key of node 0
+};
+template <int NRG>
+struct ScoreRows<NRG, SC_NONE> {};
+
+// Fills them in; a tree's rows see no key past the context by their bound.
+template <int NRG, int SC>
+__device__ __forceinline__ void load_score_rows(const AttnParams &p, int h, int q0, int nq, int row0, int sl, int qa,
+                                                int i16, ScoreRows<NRG, SC> &sr, int (&lim)[NRG]) {
+    sr.cap = p.cap_log2e;
+    sr.node0 = sl - nq;
+#pragma unroll
+    for (int rg = 0; rg < NRG; ++rg) {
+        const int r = row0 + 16 * rg + i16;
+        const int j = r / p.G;
+        const bool row = r < nq * p.G;
+        sr.slope[rg] = 0.0f;
+        sr.pos[rg] = 0;
+        sr.tree[rg] = 0;
+        if constexpr (SC == SC_BIAS) {
+            if (row) {
+                sr.slope[rg] = p.slopes[h * p.G + (r - j * p.G)] * LOG2E;
+                sr.pos[rg] = qa + j;
+            }
+        } else if (p.tree && row) {
+            sr.tree[rg] = tree_row(p, q0, j);
+            lim[rg] = min(lim[rg], sl - nq - 1);
+        }
+    }
+}
+
+// attend_subpage with the scored forms.  The scores are brought to log2 units
+// (y) before the mask and the maximum.  In a masked sub-page (one that some
+// row does not see in full) the V scales are made finite, as a hidden key's
+// P = 0 does not cancel an Inf or a NaN.
+template <int NRG, int SC>
+__device__ __forceinline__ void attend_subpage_scored(WaveAcc<NRG> &acc, const SubPage &sp,
+                                                      const half8_t (&qf)[NRG][4], int tok0, int kv_end,
+                                                      const int (&lim)[NRG], const ScoreRows<NRG, SC> &sr, float c,
+                                                      int g, bool mask) {
+    half8_t ka[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const uint32_t sw = sp.ks[b >> 1];
+        const half_t d = __builtin_bit_cast(half2_t, sw)[b & 1];
+        const half8_t dd = {d, d, d, d, d, d, d, d};
+        ka[b] = i8x8_to_half8(dw(sp.kq, 2 * b), dw(sp.kq, 2 * b + 1)) * dd;
+    }
+    half2_t vs[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const uint32_t w = dw(sp.vs, b);
+        vs[b] = __builtin_bit_cast(half2_t, w);
+    }
+    if (mask) {  // uniform
+#pragma unroll
+        for (int b = 0; b < 8; ++b) vs[b] = finite2(vs[b]);
+    }
+#pragma unroll
+    for (int rg = 0; rg < NRG; ++rg) {
+        float4_t sacc = mfma16(ka[0], qf[rg][0], float4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int b = 1; b < 4; ++b) sacc = mfma16(ka[b], qf[rg][b], sacc);
+        float y[4];
+        const float kb = SC == SC_BIAS ? (float)(tok0 + 4 * g - sr.pos[rg]) * sr.slope[rg] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // token 4g + i
+            if constexpr (SC == SC_CAP) y[i] = capped(sacc[i] * c, sr.cap, 0.0f);
+            else if constexpr (SC == SC_BIAS) y[i] = fmaf(sacc[i], c, fmaf(sr.slope[rg], (float)i, kb));
+            else y[i] = sacc[i] * c;
+        }
+        if (mask) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = tok0 + 4 * g + i;
+                bool seen = key <= lim[rg];
+                if constexpr (SC != SC_BIAS) seen = seen || tree_sees(sr.tree[rg], key - sr.node0);
+                y[i] = key < kv_end && seen ? y[i] : -INFINITY;
+            }
+        }
+        const float ml = max4f(y);
+        if (__builtin_amdgcn_ballot_w64(ml > acc.m[rg] + LAZY_TAU)) {  // as in attend_subpage
+            const float mt = xrow_max(ml);
+            const bool need = mt > acc.m[rg] + LAZY_TAU;
+            const float mn = need ? mt : acc.m[rg];
+            const float alpha = need ? __builtin_amdgcn_exp2f(acc.m[rg] - mn) : 1.0f;
+            acc.m[rg] = mn;
+            acc.l[rg] *= alpha;
+#pragma unroll
+            for (int mm = 0; mm < 8; ++mm) acc.o[rg][mm] *= alpha;
+        }
+        const float nm = acc.m[rg] == -INFINITY ? 0.0f : acc.m[rg];
+        float pr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pr[i] = __builtin_amdgcn_exp2f(y[i] - nm);
+        acc.l[rg] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+        const half2_t p01 = {(half_t)pr[0], (half_t)pr[1]};
+        const half2_t p23 = {(half_t)pr[2], (half_t)pr[3]};
+        half4_t pb[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const half2_t a = p01 * vs[2 * b];
+            const half2_t c2 = p23 * vs[2 * b + 1];
+            pb[b] = half4_t{a[0], a[1], c2[0], c2[1]};
+        }
+#pragma unroll
+        for (int mm = 0; mm < 8; ++mm) {
+            half2_t lo, hi;
+            i8x4_to_f16x4(dw(sp.vq, mm), lo, hi);
+            const half4_t va = {lo[0], lo[1], hi[0], hi[1]};
+            acc.o[rg][mm] = mfma16k16(va, pb[mm >> 1], acc.o[rg][mm]);
+        }
+    }
+}
+
 // Loads the Q^T fragments and per-row causal bounds for rows row0 + 16*rg + i16.
 template <int NRG, int QDT>
 __device__ __forceinline__ void load_rows(const AttnParams &p, int h, int q0, int nrows, int row0,
@@ -407,11 +572,11 @@ __device__ __forceinline__ void load_rows(const AttnParams &p, int h, int q0, in
 // and a sub-page's address is scalar arithmetic (no division per sub-page).
 // j0 / jstep: the wave takes sub-pages j0, j0 + jstep, ... of the range (the
 // waves of a workgroup interleave over one range).
-template <int NRG, bool NT, int DEPTH>
+template <int NRG, bool NT, int DEPTH, int SC = SC_NONE>
 __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams &p, int s, int h,
                                              int wb, int we, const half8_t (&qf)[NRG][4],
-                                             const int (&lim)[NRG], int lane, int i16, int g,
-                                             int j0 = 0, int jstep = 1) {
+                                             const int (&lim)[NRG], const ScoreRows<NRG, SC> &sr, int lane, int i16,
+                                             int g, int j0 = 0, int jstep = 1) {
     const int nall = (we - wb + 15) >> 4;
     const int nsub = nall > j0 ? (nall - j0 + jstep - 1) / jstep : 0;  // this wave's sub-pages
     if (nsub <= 0) return;
@@ -468,8 +633,9 @@ __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams
             if (j < nsub) {  // uniform
                 fetch(buf[(u + DEPTH - 1) % DEPTH], j + DEPTH - 1);
                 const int tok0 = wb + 16 * (j0 + jstep * j);
-                attend_subpage<NRG>(acc, buf[u], qf, tok0, we, lim, c, g,
-                                    !(tok0 + 16 <= we && tok0 + 15 <= lim_min));
+                const bool mask = !(tok0 + 16 <= we && tok0 + 15 <= lim_min);
+                if constexpr (SC == SC_NONE) attend_subpage<NRG>(acc, buf[u], qf, tok0, we, lim, c, g, mask);
+                else attend_subpage_scored<NRG, SC>(acc, buf[u], qf, tok0, we, lim, sr, c, g, mask);
             }
         }
     }
@@ -526,11 +692,11 @@ static_assert(SUBPAGE_BYTES == 2 * 1024 + 128, "two full copies and an 8-lane on
 // is computed, so DEPTH - 1 sub-pages are in flight per wave with no
 // registers held for them.  The slot a copy fills was read into registers
 // (and consumed) in the previous step.
-template <int NRG, int DEPTH>
+template <int NRG, int DEPTH, int SC = SC_NONE>
 __device__ __forceinline__ void stream_range_lds(WaveAcc<NRG> &acc, const AttnParams &p, int s, int h,
                                                  int wb, int we, const half8_t (&qf)[NRG][4],
-                                                 const int (&lim)[NRG], int lane, int i16, int g, int j0,
-                                                 int jstep, uint8_t *ring) {
+                                                 const int (&lim)[NRG], const ScoreRows<NRG, SC> &sr, int lane, int i16,
+                                                 int g, int j0, int jstep, uint8_t *ring) {
     const int nall = (we - wb + 15) >> 4;
     const int nsub = nall > j0 ? (nall - j0 + jstep - 1) / jstep : 0;  // this wave's sub-pages
     if (nsub <= 0) return;
@@ -624,8 +790,9 @@ __device__ __forceinline__ void stream_range_lds(WaveAcc<NRG> &acc, const AttnPa
                 sp.vs[0] = *reinterpret_cast<const u32x4 *>(sb + SUBPAGE_BYTES + lo.vs);
                 sp.vs[1] = *reinterpret_cast<const u32x4 *>(sb + SUBPAGE_BYTES + lo.vs + 16);
                 const int tok0 = wb + 16 * (j0 + jstep * j);
-                attend_subpage<NRG>(acc, sp, qf, tok0, we, lim, c, g,
-                                    !(tok0 + 16 <= we && tok0 + 15 <= lim_min));
+                const bool mask = !(tok0 + 16 <= we && tok0 + 15 <= lim_min);
+                if constexpr (SC == SC_NONE) attend_subpage<NRG>(acc, sp, qf, tok0, we, lim, c, g, mask);
+                else attend_subpage_scored<NRG, SC>(acc, sp, qf, tok0, we, lim, sr, c, g, mask);
             }
         }
     }
@@ -869,7 +1036,7 @@ constexpr int dec_nw(int nrg, bool chunk) { return nrg == 2 && !chunk ? 8 : DEC_
 #endif
 constexpr int dec_pad(int nrg, bool chunk) { return nrg == 2 && !chunk ? GFA_DEC_PAD8 : GFA_DEC_PAD; }
 
-template <int NRG, int QDT, int ODT, bool CHUNK = false>
+template <int NRG, int QDT, int ODT, bool CHUNK = false, int SC = SC_NONE>
 __global__ __launch_bounds__(64 * dec_nw(NRG, CHUNK))
 __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void attn_decode_kernel(AttnParams p) {
     constexpr int NW = dec_nw(NRG, CHUNK);  // waves in this workgroup
@@ -1070,16 +1237,18 @@ __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void at
         half8_t qf[NRG][4];
         int lim[NRG];
         load_rows<NRG, QDT>(p, h, si.q0, nrows, rc, si.sl, si.qa, i16, g, qf, lim);
+        ScoreRows<NRG, SC> sr;
+        if constexpr (SC != SC_NONE) load_score_rows<NRG, SC>(p, h, si.q0, si.nq, rc, si.sl, si.qa, i16, sr, lim);
         WaveAcc<NRG> acc;
         acc_init(acc);
         if constexpr (NRG >= 2) {  // verify tiles: sub-pages staged through this wave's sm_o slice
             static_assert(sizeof(sm_o[0]) >= DEC_RING * DEC_RING_SLOT, "ring fits the wave's slice");
-            stream_range_lds<NRG, DEC_RING>(acc, p, s, h, 16 * a, min(16 * b, si.kv_lim), qf, lim, lane, i16,
-                                            g, j0, jstep, reinterpret_cast<uint8_t *>(&sm_o[wv][0][0]));
+            stream_range_lds<NRG, DEC_RING, SC>(acc, p, s, h, 16 * a, min(16 * b, si.kv_lim), qf, lim, sr, lane, i16,
+                                                g, j0, jstep, reinterpret_cast<uint8_t *>(&sm_o[wv][0][0]));
         } else {
-            stream_range<NRG, GFA_DEC_NT != 0, DecCfg<NRG>::depth>(acc, p, s, h, 16 * a,
-                                                                     min(16 * b, si.kv_lim), qf, lim,
-                                                                     lane, i16, g, j0, jstep);
+            stream_range<NRG, GFA_DEC_NT != 0, DecCfg<NRG>::depth, SC>(acc, p, s, h, 16 * a,
+                                                                         min(16 * b, si.kv_lim), qf, lim, sr,
+                                                                         lane, i16, g, j0, jstep);
         }
         // ---- merge the chunk's waves' states in LDS ------------------------
         // in passes of 32 rows (row groups 2*ps, 2*ps + 1): a wave's LDS
@@ -1458,13 +1627,6 @@ __device__ __forceinline__ half8_t scale8_f32(half8_t v, float s) {
     return r;
 }
 
-// fp16 pair with Inf / NaN replaced by +-65504 (v_pk_max/min_f16 return the
-// non-NaN operand).
-__device__ __forceinline__ half2_t finite2(half2_t x) {
-    const half2_t hi = {(half_t)65504.0f, (half_t)65504.0f};
-    return __builtin_elementwise_min(__builtin_elementwise_max(x, -hi), hi);
-}
-
 // Dequantizes the lane's raw half sub-page into the LDS stages (sub-page sp
 // of the tile): K^ rows into kst, V^T columns into vst.  TAIL (the last tile
 // of the range, the only one that can hold keys past kv_end): bytes of tokens
@@ -1526,7 +1688,7 @@ __device__ __forceinline__ void pf_dequant_v(const PfRaw &r, uint8_t *vst, int s
 // them there), whose V rows are the caller's own.  An instance of its own: the
 // clearing of unseen V in the paged instance's copy loop cost the 32K prompt
 // 1 % (11.07 -> 11.2 ms), though it never ran there.
-template <int QDT, int ODT, bool VF16, bool MASK, int KS = 1, bool FLAT = false>
+template <int QDT, int ODT, bool VF16, bool MASK, int KS = 1, bool FLAT = false, int SC = SC_NONE>
 __global__ __launch_bounds__(64 * PF_WAVES)
 __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p) {
     static_assert(KS == 1 || KS == 2, "256-row tiles, or 128-row key-interleaved tiles");
@@ -1729,7 +1891,9 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
         };
         auto dequant_v = [&](const PfRawT &rw, int t, auto tail) __attribute__((always_inline)) {
             uint8_t *vst = ldsv + (t % NSTAGE) * PF_VBYTES;
-            constexpr bool T = decltype(tail)::value;
+            // (a scored form may hide keys of the tiles before the last: its V
+            // scales are made finite in every tile)
+            constexpr bool T = decltype(tail)::value || SC != SC_NONE;
             pf_dequant_v<T, VF16>(rw.h[0], vst, wsp, lane, 0);
             pf_dequant_v<T, VF16>(rw.h[1], vst, wsp, lane, 1);
         };
@@ -1870,7 +2034,7 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
     const bool rvalid = r < nrows;
     const int j = rvalid ? fdiv(r, p.g_div) : 0;
     const int hq = h * p.G + (rvalid ? r - j * p.G : 0);
-    const int lim = rvalid ? (p.causal ? min(sl - 1, qa + j) : sl - 1) : INT32_MAX;
+    int lim = rvalid ? (p.causal ? min(sl - 1, qa + j) : sl - 1) : INT32_MAX;
     const bool wact = row0 + 32 * cw < nrows;  // uniform over the wave (and its KS = 2 partner)
     if (!wact) {
         // all 32 rows past the sequence's rows (its last row tile): keep the
@@ -1913,6 +2077,18 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
             if (!rvalid) qf[kk] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
         }
     }
+    // the scored forms' row: see ScoreRows
+    [[maybe_unused]] uint64_t tree = 0;
+    [[maybe_unused]] const int node0 = sl - nq;
+    [[maybe_unused]] float slope = 0.0f;
+    if constexpr (SC == SC_BIAS) {
+        slope = rvalid ? p.slopes[hq] * LOG2E : 0.0f;
+    } else if constexpr (SC != SC_NONE) {
+        if (p.tree && rvalid) {
+            tree = tree_row(p, q0, j);
+            lim = min(lim, node0 - 1);
+        }
+    }
     int lim_min;  // smallest bound over the wave's rows: tiles below it need no mask
     {
         const float f = (float)min(lim, 1 << 24);
@@ -1942,7 +2118,8 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
     // exponentials and PV MFMAs.
     float16v_t sacc[PF_NST];  // S' of the tile between its two half-steps
     // S'^T = K^ . Q^T - m for the 32-key subtiles of the tile (stage kst)
-    auto qk = [&](const uint8_t *kst) __attribute__((always_inline)) {
+    // (kt: the tile, for the distance bias)
+    auto qk = [&]([[maybe_unused]] int kt, const uint8_t *kst) __attribute__((always_inline)) {
         // -m in all 16 accumulator registers, the srcC of the first MFMA of
         // both chains.  Each 64-bit pair passes through an empty asm so that
         // the compiler copies it with one v_mov_b64 (7 moves, against 15
@@ -1962,7 +2139,17 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
         }
 #pragma unroll
         for (int st = 0; st < PF_NST; ++st) {
-            sacc[st] = msp;
+            if constexpr (SC == SC_CAP) {  // m is not linear in the capped score: it is subtracted in sv
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sacc[st][e] = 0.0f;
+            } else if constexpr (SC == SC_BIAS) {
+                // the bias of the lane's 16 keys with -m: register e's key is 8 (e / 4) + e % 4 past the first
+                const float b0 = fmaf(slope, (float)(PF_TK * (kt + ktb) + 32 * st + 4 * hb - (qa + j)), -m_use);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sacc[st][e] = fmaf(slope, (float)(8 * (e >> 2) + (e & 3)), b0);
+            } else {
+                sacc[st] = msp;
+            }
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
                 const half8_t a = *reinterpret_cast<const half8_t *>(kst + kread + 32 * st * PF_KPITCH + 32 * kk);
@@ -2012,13 +2199,21 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
                     }
             }
         }
+        if constexpr (SC == SC_CAP) {  // (a product of 2 log2 e * scale / cap came out of the QK)
+#pragma unroll
+            for (int st = 0; st < PF_NST; ++st)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sacc[st][e] = capped(sacc[st][e], p.cap_log2e, m_use);
+        }
         if (kbase_t + PF_TK - 1 > lim_min) {  // uniform: tile crosses some row's bound
 #pragma unroll
             for (int st = 0; st < PF_NST; ++st)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int key = kbase_t + 32 * st + 8 * (e >> 2) + 4 * hb + (e & 3);
-                    sacc[st][e] = key <= lim ? sacc[st][e] : -INFINITY;
+                    bool seen = key <= lim;
+                    if constexpr (SC == SC_TREE || SC == SC_CAP) seen = seen || tree_sees(tree, key - node0);
+                    sacc[st][e] = seen ? sacc[st][e] : -INFINITY;
                 }
         }
         // The lane's own max over its 32 keys, as a tree of depth 4.  A row's
@@ -2077,7 +2272,7 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
     if constexpr (KS == 1) {
         if (grp) __syncthreads();  // half-step 0
         for (int kt = 0, stg = 0; kt < ntk; ++kt, stg = stg == NSTAGE - 1 ? 0 : stg + 1) {
-            qk(ldsk + stg * PF_KBYTES);
+            qk(kt, ldsk + stg * PF_KBYTES);
             __syncthreads();
             sv(kt, ldsv + stg * PF_VBYTES);
             __syncthreads();
@@ -2091,7 +2286,7 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
         const uint8_t *kst = ldsk + grp * PF_KBYTES;
         const uint8_t *vst = ldsv + grp * PF_VBYTES;
         for (int kt = grp; kt < ntk; kt += 2) {
-            qk(kst);
+            qk(kt, kst);
             __syncthreads();
             sv(kt, vst);
             __syncthreads();
@@ -3568,7 +3763,7 @@ void set_prefill_ws(AttnParams &p, const Plan &pl, char *ws) {
     p.pf_img_seq = 0;
 }
 
-template <int QDT, int ODT>
+template <int QDT, int ODT, int SC = SC_NONE>
 hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_seqs, int num_kv_heads,
                       int max_query_len, hipStream_t stream) {
     AttnParams p = p0;
@@ -3588,7 +3783,7 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
         // combine rows: a split segment has at most min(max_query_len * G, slot) rows
         const int crow = max(1, min(max_query_len * p.G, c.rows_hi));
         if (c.nrg == 1) {
-            attn_decode_kernel<1, QDT, ODT><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
+            attn_decode_kernel<1, QDT, ODT, false, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
             // short contexts with few pieces per segment at most (resident
             // workgroups over segments): one merging workgroup per segment.
             // There the merge launch is mostly workgroups that find their
@@ -3599,14 +3794,14 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
             else
                 attn_combine_kernel<1, ODT><<<dim3(num_seqs, num_kv_heads, crow), 256, 0, stream>>>(pd);
         } else if (c.nrg == 3) {
-            attn_decode_kernel<3, QDT, ODT><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
+            attn_decode_kernel<3, QDT, ODT, false, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
             attn_combine_kernel<3, ODT><<<dim3(num_seqs, num_kv_heads, crow), 256, 0, stream>>>(pd);
         } else {
-            if (c.rows_hi > 32) attn_decode_kernel<2, QDT, ODT, true><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
+            if (c.rows_hi > 32) attn_decode_kernel<2, QDT, ODT, true, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
             else {  // one 8-wave workgroup where the plan sized two 4-wave ones
                 constexpr int nw = dec_nw(2, false);
                 pd.nwg = c.nwg * DEC_NW / nw;
-                attn_decode_kernel<2, QDT, ODT><<<pd.nwg, 64 * nw, 0, stream>>>(pd);
+                attn_decode_kernel<2, QDT, ODT, false, SC><<<pd.nwg, 64 * nw, 0, stream>>>(pd);
             }
             // (a mixed batch's class mostly finds nothing to merge: 250 prompts
             // of 30 tokens at 48/8 128 us with a launch per row, 89.5 per segment)
@@ -3625,11 +3820,11 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
         const int tiles = (rows + pl.pf_rows - 1) / pl.pf_rows;
         const dim3 grid = p.pf_items ? dim3(pl.pf_grid_items * num_kv_heads) : dim3(tiles * num_kv_heads, num_seqs);
         if (p.mask) {  // (padded batches: fp32 output, 256-row tiles)
-            if constexpr (ODT == GFA_DTYPE_F32)
+            if constexpr (ODT == GFA_DTYPE_F32 && SC == SC_NONE)
                 attn_prefill_kernel<QDT, ODT, false, true><<<grid, 64 * PF_WAVES, 0, stream>>>(p);
         } else if (pl.pf_rows == PF_ROWS)
-            attn_prefill_kernel<QDT, ODT, false, false><<<grid, 64 * PF_WAVES, 0, stream>>>(p);
-        else attn_prefill_kernel<QDT, ODT, false, false, 2><<<grid, 64 * PF_WAVES, 0, stream>>>(p);
+            attn_prefill_kernel<QDT, ODT, false, false, 1, false, SC><<<grid, 64 * PF_WAVES, 0, stream>>>(p);
+        else attn_prefill_kernel<QDT, ODT, false, false, 2, false, SC><<<grid, 64 * PF_WAVES, 0, stream>>>(p);
         if (p.pf_items && pl.pf_slots_max)  // returns at once when the plan split nothing
             attn_prefill_combine_kernel<ODT><<<device_cus() * GFA_PFC_WGS_PER_CU, 256, 0, stream>>>(p);
     }
@@ -3761,6 +3956,24 @@ struct NewKV {
     const int64_t *slot_mapping;
 };
 
+// A scored call's forms: cap 0, slopes or tree nullptr where they are absent.
+struct Scores {
+    float cap;
+    const float *slopes;
+    const int64_t *tree;
+};
+
+template <int SC>
+hipError_t launch_scored(const AttnParams &p, const Plan &pl, char *ws, int q_dtype, int out_dtype,
+                         int max_query_len, hipStream_t stream) {
+    const bool f32 = out_dtype == GFA_DTYPE_F32;
+    if (q_dtype == GFA_DTYPE_F16)
+        return f32 ? launch_all<GFA_DTYPE_F16, GFA_DTYPE_F32, SC>(p, pl, ws, p.num_seqs, p.Hkv, max_query_len, stream)
+                   : launch_all<GFA_DTYPE_F16, GFA_DTYPE_F16, SC>(p, pl, ws, p.num_seqs, p.Hkv, max_query_len, stream);
+    return f32 ? launch_all<GFA_DTYPE_BF16, GFA_DTYPE_F32, SC>(p, pl, ws, p.num_seqs, p.Hkv, max_query_len, stream)
+               : launch_all<GFA_DTYPE_BF16, GFA_DTYPE_BF16, SC>(p, pl, ws, p.num_seqs, p.Hkv, max_query_len, stream);
+}
+
 hipError_t paged_attention_impl(
     const void *q, int q_dtype, int64_t q_token_stride, int64_t q_head_stride,
     const uint8_t *k_cache, const uint8_t *v_cache, int64_t cache_block_stride,
@@ -3769,7 +3982,8 @@ hipError_t paged_attention_impl(
     int causal, int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int head_size,
     int block_size, int max_query_len, int max_seq_len, float scale, void *out, int out_dtype,
     int64_t out_token_stride, int64_t out_head_stride, void *workspace, size_t workspace_bytes,
-    const NewKV *nkv, hipStream_t stream, bool noalloc = false, const Padded *padded = nullptr) {
+    const NewKV *nkv, hipStream_t stream, bool noalloc = false, const Padded *padded = nullptr,
+    const Scores *scores = nullptr) {
     if (nkv && num_tokens > 0) {
         const uint64_t align = nkv->dtype == GFA_DTYPE_F32 ? 8 : 4;  // two values per lane
         if (nkv->dtype != q_dtype ||
@@ -3865,7 +4079,10 @@ hipError_t paged_attention_impl(
     p.Hkv = num_kv_heads;
     p.G = G;
     p.block_size = block_size;
-    p.scale_log2e = scale * LOG2E;
+    p.scale_log2e = scores && scores->cap > 0.0f ? scale * (2.0f * LOG2E / scores->cap) : scale * LOG2E;
+    p.cap_log2e = scores ? scores->cap * LOG2E : 0.0f;
+    p.slopes = scores ? scores->slopes : nullptr;
+    p.tree = scores ? scores->tree : nullptr;
     set_prefill_scale(p);
     set_divisors(p);
     p.out = out;
@@ -3915,6 +4132,11 @@ hipError_t paged_attention_impl(
         }
     }
 
+    if (scores) {
+        if (scores->cap > 0.0f) return launch_scored<SC_CAP>(p, pl, ws, q_dtype, out_dtype, max_query_len, stream);
+        if (scores->slopes) return launch_scored<SC_BIAS>(p, pl, ws, q_dtype, out_dtype, max_query_len, stream);
+        if (scores->tree) return launch_scored<SC_TREE>(p, pl, ws, q_dtype, out_dtype, max_query_len, stream);
+    }
 #define GFA_DISPATCH_O(QDT)                                                                    \
     switch (out_dtype) {                                                                       \
         case GFA_DTYPE_F32: return launch_all<QDT, GFA_DTYPE_F32>(p, pl, ws, num_seqs, num_kv_heads, max_query_len, stream); \
@@ -4014,6 +4236,46 @@ extern "C" hipError_t gfx906_fa_amd_paged_attention_kv_write(
                                 num_heads, num_kv_heads, head_size, block_size, max_query_len, max_seq_len,
                                 scale, out, out_dtype, out_token_stride, out_head_stride, workspace,
                                 workspace_bytes, &nkv, stream);
+}
+
+extern "C" hipError_t gfx906_fa_amd_scored_paged_attention(
+    const void *q, int q_dtype, int64_t q_token_stride, int64_t q_head_stride,
+    const uint8_t *k_cache, const uint8_t *v_cache, int64_t cache_block_stride,
+    int64_t cache_head_stride, const int32_t *block_table, int64_t block_table_stride,
+    const int32_t *seq_lens, const int32_t *query_start_loc, const int32_t *q_abs_offset,
+    int causal, float soft_cap, const float *alibi_slopes, const int64_t *tree_mask,
+    int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int head_size,
+    int block_size, int max_query_len, int max_seq_len, float scale, void *out, int out_dtype,
+    int64_t out_token_stride, int64_t out_head_stride, void *workspace, size_t workspace_bytes,
+    hipStream_t stream) {
+    if (!(soft_cap >= 0.0f) || (soft_cap > 0.0f && !std::isfinite(scale * (2.0f * LOG2E / soft_cap))) ||
+        !std::isfinite(soft_cap * LOG2E)) {
+        fprintf(stderr, "[gfx906_fa_amd] scored_paged_attention: soft_cap must be 0 or positive, finite and no "
+                        "smaller than the scale allows (got %g)\n", (double)soft_cap);
+        return hipErrorInvalidValue;
+    }
+    if (alibi_slopes && (soft_cap > 0.0f || tree_mask)) {
+        fprintf(stderr, "[gfx906_fa_amd] scored_paged_attention: alibi_slopes exclude soft_cap and tree_mask\n");
+        return hipErrorInvalidValue;
+    }
+    if (tree_mask && (q_abs_offset || !causal || max_query_len > 64)) {
+        fprintf(stderr, "[gfx906_fa_amd] scored_paged_attention: a tree is causal, without q_abs_offset, of at most "
+                        "64 nodes (max_query_len %d)\n", max_query_len);
+        return hipErrorInvalidValue;
+    }
+    const bool scored = soft_cap > 0.0f || alibi_slopes || tree_mask;
+    if (scored && ((q_dtype != GFA_DTYPE_F16 && q_dtype != GFA_DTYPE_BF16) ||
+                   (out_dtype != q_dtype && out_dtype != GFA_DTYPE_F32))) {
+        fprintf(stderr, "[gfx906_fa_amd] scored_paged_attention: query must be fp16 or bf16, out of its type or fp32\n");
+        return hipErrorInvalidValue;
+    }
+    const Scores sc{soft_cap, alibi_slopes, tree_mask};
+    return paged_attention_impl(q, q_dtype, q_token_stride, q_head_stride, k_cache, v_cache,
+                                cache_block_stride, cache_head_stride, block_table, block_table_stride,
+                                seq_lens, query_start_loc, q_abs_offset, causal, num_seqs, num_tokens,
+                                num_heads, num_kv_heads, head_size, block_size, max_query_len, max_seq_len,
+                                scale, out, out_dtype, out_token_stride, out_head_stride, workspace,
+                                workspace_bytes, nullptr, stream, false, nullptr, scored ? &sc : nullptr);
 }
 
 namespace {

@@ -314,31 +314,223 @@ void launch_rope(const RopeArgs &a, bool neox, unsigned grid, hipStream_t stream
     else q8_rope_cache_write_kernel<DT, CSDT, false><<<grid, 256, 0, stream>>>(a);
 }
 
-}  // namespace
+// ---------------------------------------------------------------------------
+// RMS norms of the query and key heads, then the rotation, then the cache
+// write.  Per head row x of 128 values:
+//   y = x * rsqrt(mean(x^2) + eps) * w,  then for each rotated pair of y
+//   (u, v):  u' = u cos - v sin,  v' = v cos + u sin,
+// all in fp32, rounded once to the model dtype as the row is stored.  The
+// quantized key is the stored one, so the cache holds what the unfused path
+// would write.  A position outside [0, max_position) is normed, not rotated.
+// Work mapping as above; the sum of squares is over the 16 lanes of a row.
 
-extern "C" hipError_t gfx906_fa_amd_rope_cache_write_kv(
+// The lane's 8 key and value ints (columns 8 i ..) of kv-head h at a slot, and
+// each block's scales from the first lane of its quad.
+__device__ __forceinline__ void store_row_chunk(const RopeArgs &a, int64_t slot, int h, int i, uint32_t klo, uint32_t khi,
+                                                float dk, uint32_t vlo, uint32_t vhi, float dv) {
+    const int d0 = 8 * i;
+    const int64_t page = slot / a.block_size;
+    const int off = (int)(slot - page * a.block_size);
+    const int tt = off & 15, b = d0 >> 5, m = d0 >> 4;
+    const int64_t base = page * a.cbs + (int64_t)h * a.chs + (int64_t)(off >> 4) * SUBPAGE_BYTES;
+    *reinterpret_cast<u32x2 *>(a.kc + base + (b >> 1) * 1024 + (4 * tt + ((d0 >> 3) & 3)) * 16 + (b & 1) * 8) =
+        u32x2{klo, khi};
+    uint8_t *vrow = a.vc + base + (m >> 2) * 1024 + (tt >> 2) * 256 + (tt & 3) + (m & 3) * 4 + (d0 & 15) * 16;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vrow[e * 16] = (uint8_t)((e < 4 ? vlo : vhi) >> (8 * (e & 3)));
+    if ((i & 3) == 0) {
+        *reinterpret_cast<uint16_t *>(a.kc + base + SCALE_OFF + (4 * tt + b) * 2) = f32_to_half_bits(dk);
+        *reinterpret_cast<uint16_t *>(a.vc + base + SCALE_OFF + ((tt >> 2) * 4 + b) * 8 + (tt & 3) * 2) =
+            f32_to_half_bits(dv);
+    }
+}
+
+struct NormArgs {
+    RopeArgs r;
+    const void *wq, *wk;
+    float eps;
+};
+
+__device__ __forceinline__ float row16_sum(float v) {
+    v += dpp_f32<DPP_QUAD_XOR1>(v);
+    v += dpp_f32<DPP_QUAD_XOR2>(v);
+    v += dpp_f32<DPP_ROW_HALF_MIRROR>(v);
+    v += dpp_f32<DPP_ROW_MIRROR>(v);
+    return v;
+}
+
+// fp32 -> model dtype, nearest even (a NaN stays one)
+template <int DT>
+__device__ __forceinline__ uint32_t round_el(float v) {
+    if constexpr (DT == GFA_DTYPE_F16) return f32_to_half_bits(v);
+    else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+// 8 consecutive values of a 16-byte aligned row chunk of type T2, exact in fp32
+template <int T2>
+__device__ __forceinline__ void load8_f32(const void *row, int col, float (&v)[8]) {
+    if constexpr (T2 == GFA_DTYPE_F32) {
+        const float4_t *p = reinterpret_cast<const float4_t *>(static_cast<const float *>(row) + col);
+        const float4_t a = p[0], b = p[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = a[e];
+            v[4 + e] = b[e];
+        }
+    } else {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(row) + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[2 * e] = el_to_f32<T2>(w[e] & 0xFFFFu);
+            v[2 * e + 1] = el_to_f32<T2>(w[e] >> 16);
+        }
+    }
+}
+
+// n consecutive cos or sin values in fp32, 8-byte aligned
+template <int CSDT, int N>
+__device__ __forceinline__ void load_cs_f32(const void *row, int col, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) load2_as_f32<CSDT>(row, col + e, v[e], v[e + 1]);
+}
+
+template <int DT, int CSDT, bool NEOX>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q8_norm_rope_cache_write_kernel(NormArgs n) {
+    const RopeArgs &a = n.r;
+    const int64_t wave = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int i = lane & 15, g = lane >> 4;
+    const int d0 = 8 * i;
+    const int64_t t = wave / a.nchunk;
+    if (t >= a.num_tokens) return;  // uniform over the wave
+    const int c0 = 4 * ROPE_ITERS * (int)(wave - t * a.nchunk);
+    const int R = a.Hq + a.Hkv;
+    u32x4_t xw[ROPE_ITERS], vw[ROPE_ITERS];
+#pragma unroll
+    for (int it = 0; it < ROPE_ITERS; ++it) {
+        xw[it] = u32x4_t{0, 0, 0, 0};
+        vw[it] = u32x4_t{0, 0, 0, 0};
+        const int row = c0 + 4 * it + g;
+        if (row < a.Hq) {
+            xw[it] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(a.q) + t * a.qts +
+                                                      (int64_t)row * a.qhs + d0);
+        } else if (row < R) {
+            const int h = row - a.Hq;
+            xw[it] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(a.k) + t * a.kts +
+                                                      (int64_t)h * a.khs + d0);
+            vw[it] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(a.v) + t * a.vts +
+                                                      (int64_t)h * a.vhs + d0);
+        }
+    }
+    const int64_t pos = a.pos[t];
+    const int64_t slot = a.slot[t];
+    const bool turn = pos >= 0 && pos < a.max_pos && d0 < a.rot;
+    const int half = a.rot >> 1;
+    // unrotated values: cos 1, sin 0
+    float c[8] = {1, 1, 1, 1, 1, 1, 1, 1}, s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (turn) {
+        const void *csrow = static_cast<const char *>(a.cs) + pos * a.cs_stride * (CSDT == GFA_DTYPE_F32 ? 4 : 2);
+        if constexpr (NEOX) {
+            const int col = d0 < half ? d0 : d0 - half;
+            load_cs_f32<CSDT, 8>(csrow, col, c);
+            load_cs_f32<CSDT, 8>(csrow, half + col, s);
+        } else {
+            load_cs_f32<CSDT, 4>(csrow, d0 >> 1, c);
+            load_cs_f32<CSDT, 4>(csrow, half + (d0 >> 1), s);
+        }
+    }
+    // (neox) the lane that holds the pair's other value, and the sign of its sin
+    const int src = d0 < half ? lane + (half >> 3) : (d0 < a.rot ? lane - (half >> 3) : lane);
+    const bool first = d0 < half;
+    float wq[8], wk[8];
+    load8_f32<DT>(n.wq, d0, wq);
+    load8_f32<DT>(n.wk, d0, wk);
+#pragma unroll
+    for (int it = 0; it < ROPE_ITERS; ++it) {
+        if (c0 + 4 * it >= R) break;  // uniform: no row of this iteration exists
+        const int row = c0 + 4 * it + g;
+        const bool active = row < R;  // the same for the 16 lanes of a row
+        const bool is_q = row < a.Hq;
+        float x[8], ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[2 * e] = el_to_f32<DT>(xw[it][e] & 0xFFFFu);
+            x[2 * e + 1] = el_to_f32<DT>(xw[it][e] >> 16);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+        const float inv = __builtin_amdgcn_rsqf(row16_sum(ss) * (1.0f / 128.0f) + n.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (is_q ? wq[e] : wk[e]);
+        if constexpr (NEOX) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = __shfl(x[e], src);
+                x[e] = first ? x[e] * c[e] - p * s[e] : x[e] * c[e] + p * s[e];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float u = x[2 * j], v = x[2 * j + 1];
+                x[2 * j] = u * c[j] - v * s[j];
+                x[2 * j + 1] = v * c[j] + u * s[j];
+            }
+        }
+        u32x4_t w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = round_el<DT>(x[2 * e]) | (round_el<DT>(x[2 * e + 1]) << 16);
+        if (!active) continue;
+        uint16_t *dst = is_q ? static_cast<uint16_t *>(a.q) + t * a.qts + (int64_t)row * a.qhs + d0
+                             : static_cast<uint16_t *>(a.k) + t * a.kts + (int64_t)(row - a.Hq) * a.khs + d0;
+        *reinterpret_cast<u32x4_t *>(dst) = w;
+        if (is_q) continue;
+        float vv[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[2 * e] = el_to_f32<DT>(w[e] & 0xFFFFu);
+            x[2 * e + 1] = el_to_f32<DT>(w[e] >> 16);
+            vv[2 * e] = el_to_f32<DT>(vw[it][e] & 0xFFFFu);
+            vv[2 * e + 1] = el_to_f32<DT>(vw[it][e] >> 16);
+        }
+        uint32_t klo, khi, vlo, vhi;
+        const float dk = quant8(x, klo, khi);
+        const float dv = quant8(vv, vlo, vhi);
+        if (slot < 0) continue;
+        store_row_chunk(a, slot, row - a.Hq, i, klo, khi, dk, vlo, vhi, dv);
+    }
+}
+
+template <int DT, int CSDT>
+void launch_norm_rope(const NormArgs &a, bool neox, unsigned grid, hipStream_t stream) {
+    if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true><<<grid, 256, 0, stream>>>(a);
+    else q8_norm_rope_cache_write_kernel<DT, CSDT, false><<<grid, 256, 0, stream>>>(a);
+}
+
+// Checks an entry's arguments and fills in the kernel's; grid 0: nothing to do.
+hipError_t rope_args(
+    const char *what, RopeArgs &a, unsigned &grid,
     void *query, void *key, const void *value, int dtype, const int64_t *positions,
     const void *cos_sin_cache, int cos_sin_dtype, int64_t cos_sin_stride, int max_position,
     int rot_dim, int is_neox, const int64_t *slot_mapping, uint8_t *k_cache, uint8_t *v_cache,
     int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size,
     int64_t query_token_stride, int64_t query_head_stride, int64_t key_token_stride,
     int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
-    int64_t cache_block_stride, int64_t cache_head_stride, hipStream_t stream) {
+    int64_t cache_block_stride, int64_t cache_head_stride) {
     if (head_size != 128 || block_size <= 0 || block_size % SUBPAGE != 0 || num_heads <= 0 ||
         num_kv_heads <= 0 || num_tokens < 0 || (dtype != GFA_DTYPE_F16 && dtype != GFA_DTYPE_BF16) ||
         cos_sin_dtype < 0 || cos_sin_dtype > 2 || max_position <= 0) {
         fprintf(stderr,
-                "[gfx906_fa_amd] rope_cache_write_kv: need head_size 128, block_size %% 16 == 0, "
+                "[gfx906_fa_amd] %s: need head_size 128, block_size %% 16 == 0, "
                 "fp16/bf16 query/key/value, max_position > 0 (got head_size=%d block_size=%d dtype=%d)\n",
-                head_size, block_size, dtype);
+                what, head_size, block_size, dtype);
         return hipErrorInvalidValue;
     }
     if (rot_dim <= 0 || rot_dim > head_size || rot_dim % (is_neox ? 16 : 8) != 0 ||
         cos_sin_stride < rot_dim) {
         fprintf(stderr,
-                "[gfx906_fa_amd] rope_cache_write_kv: rot_dim=%d must be in (0, 128], a multiple of %d, "
+                "[gfx906_fa_amd] %s: rot_dim=%d must be in (0, 128], a multiple of %d, "
                 "and <= the cos_sin row stride (%lld)\n",
-                rot_dim, is_neox ? 16 : 8, (long long)cos_sin_stride);
+                what, rot_dim, is_neox ? 16 : 8, (long long)cos_sin_stride);
         return hipErrorInvalidValue;
     }
     // 16-byte row chunks for query / key / value, 8-byte cos / sin pairs and
@@ -351,12 +543,12 @@ extern "C" hipError_t gfx906_fa_amd_rope_cache_write_kv(
         (((uintptr_t)k_cache | (uintptr_t)v_cache | (uint64_t)cache_block_stride |
           (uint64_t)cache_head_stride) & 7u)) {
         fprintf(stderr,
-                "[gfx906_fa_amd] rope_cache_write_kv: query/key/value rows must start 16-byte aligned "
-                "(bases 16-aligned, strides multiples of 8 elements), cos_sin rows and the cache 8-aligned\n");
+                "[gfx906_fa_amd] %s: query/key/value rows must start 16-byte aligned "
+                "(bases 16-aligned, strides multiples of 8 elements), cos_sin rows and the cache 8-aligned\n", what);
         return hipErrorInvalidValue;
     }
+    grid = 0;
     if (num_tokens == 0) return hipSuccess;
-    RopeArgs a;
     a.q = query;
     a.k = key;
     a.v = value;
@@ -384,10 +576,32 @@ extern "C" hipError_t gfx906_fa_amd_rope_cache_write_kv(
     const int64_t waves = (int64_t)num_tokens * a.nchunk;
     const int64_t blocks = (waves + 3) / 4;
     if (blocks > 0x7FFFFFFF) {
-        fprintf(stderr, "[gfx906_fa_amd] rope_cache_write_kv: too many rows\n");
+        fprintf(stderr, "[gfx906_fa_amd] %s: too many rows\n", what);
         return hipErrorInvalidValue;
     }
-    const unsigned grid = (unsigned)blocks;
+    grid = (unsigned)blocks;
+    return hipSuccess;
+}
+
+}  // namespace
+
+extern "C" hipError_t gfx906_fa_amd_rope_cache_write_kv(
+    void *query, void *key, const void *value, int dtype, const int64_t *positions,
+    const void *cos_sin_cache, int cos_sin_dtype, int64_t cos_sin_stride, int max_position,
+    int rot_dim, int is_neox, const int64_t *slot_mapping, uint8_t *k_cache, uint8_t *v_cache,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size,
+    int64_t query_token_stride, int64_t query_head_stride, int64_t key_token_stride,
+    int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+    int64_t cache_block_stride, int64_t cache_head_stride, hipStream_t stream) {
+    RopeArgs a;
+    unsigned grid;
+    const hipError_t e =
+        rope_args("rope_cache_write_kv", a, grid, query, key, value, dtype, positions, cos_sin_cache, cos_sin_dtype, cos_sin_stride,
+                         max_position, rot_dim, is_neox, slot_mapping, k_cache, v_cache, num_tokens, num_heads,
+                         num_kv_heads, head_size, block_size, query_token_stride, query_head_stride,
+                         key_token_stride, key_head_stride, value_token_stride, value_head_stride,
+                         cache_block_stride, cache_head_stride);
+    if (e != hipSuccess || grid == 0) return e;
     const bool neox = is_neox != 0;
 #define GFA_ROPE_CS(DT)                                                     \
     switch (cos_sin_dtype) {                                                \
@@ -401,5 +615,47 @@ extern "C" hipError_t gfx906_fa_amd_rope_cache_write_kv(
         GFA_ROPE_CS(GFA_DTYPE_BF16)
     }
 #undef GFA_ROPE_CS
+    return hipGetLastError();
+}
+
+extern "C" hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
+    void *query, void *key, const void *value, const void *query_weight, const void *key_weight,
+    float eps, int dtype, const int64_t *positions,
+    const void *cos_sin_cache, int cos_sin_dtype, int64_t cos_sin_stride, int max_position,
+    int rot_dim, int is_neox, const int64_t *slot_mapping, uint8_t *k_cache, uint8_t *v_cache,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size,
+    int64_t query_token_stride, int64_t query_head_stride, int64_t key_token_stride,
+    int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+    int64_t cache_block_stride, int64_t cache_head_stride, hipStream_t stream) {
+    NormArgs a;
+    unsigned grid;
+    const hipError_t e =
+        rope_args("qk_norm_rope_cache_write_kv", a.r, grid, query, key, value, dtype, positions, cos_sin_cache, cos_sin_dtype, cos_sin_stride,
+                         max_position, rot_dim, is_neox, slot_mapping, k_cache, v_cache, num_tokens, num_heads,
+                         num_kv_heads, head_size, block_size, query_token_stride, query_head_stride,
+                         key_token_stride, key_head_stride, value_token_stride, value_head_stride,
+                         cache_block_stride, cache_head_stride);
+    if (e != hipSuccess) return e;
+    if (!(eps >= 0.0f) || (((uintptr_t)query_weight | (uintptr_t)key_weight) & 15u)) {
+        fprintf(stderr, "[gfx906_fa_amd] qk_norm_rope_cache_write_kv: eps must be >= 0 and the weights 16-byte aligned\n");
+        return hipErrorInvalidValue;
+    }
+    if (grid == 0) return hipSuccess;
+    a.wq = query_weight;
+    a.wk = key_weight;
+    a.eps = eps;
+    const bool neox = is_neox != 0;
+#define GFA_NORM_CS(DT)                                                     \
+    switch (cos_sin_dtype) {                                                \
+        case GFA_DTYPE_F32: launch_norm_rope<DT, GFA_DTYPE_F32>(a, neox, grid, stream); break; \
+        case GFA_DTYPE_F16: launch_norm_rope<DT, GFA_DTYPE_F16>(a, neox, grid, stream); break; \
+        default: launch_norm_rope<DT, GFA_DTYPE_BF16>(a, neox, grid, stream); break;           \
+    }
+    if (dtype == GFA_DTYPE_F16) {
+        GFA_NORM_CS(GFA_DTYPE_F16)
+    } else {
+        GFA_NORM_CS(GFA_DTYPE_BF16)
+    }
+#undef GFA_NORM_CS
     return hipGetLastError();
 }

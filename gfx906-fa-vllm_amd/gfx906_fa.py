@@ -27,11 +27,20 @@ gather_paged_kv_q8q8(key_cache, value_cache, block_table, seq_lens, Sk, ...)
 paged_attention(query, key_cache, value_cache, block_table, seq_lens,
                 query_start_loc, max_query_len, max_seq_len, scale, out=None, ...)
 new_kv_cache(num_blocks, block_size, num_kv_heads, head_size=128, device=...)
+For models and decoders past plain causal attention:
+scored_paged_attention(query, ..., scale, soft_cap=0.0, alibi_slopes=None, ...)
+tree_attention(query, ..., query_start_loc, tree_mask, ..., scale, soft_cap=0.0, ...)
+tree_masks(parents)
+qk_norm_rope_and_cache_q8_kv(positions, query, key, value, query_weight, key_weight, eps,
+                             cos_sin_cache, is_neox, slot_mapping, key_cache, value_cache, ...)
+compact_draft_rows(kv_caches, block_table, seq_lens, query_start_loc, accepted, num_accepted)
+read_cache_q8_kv(slot_mapping, key_cache, value_cache, dtype, k_out=None, v_out=None)
 """
 from __future__ import annotations
 
 import ctypes
 import os
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -98,6 +107,13 @@ def _load():
                                                      I, I, I, I, I, I, I, F, P, P, SZ, P]),
         "gfx906_fa_amd_flat_attention_workspace_size": (SZ, [I, I, I, I, I, I]),
         "gfx906_fa_amd_flat_attention": (I, [P, P, P, P, P, P, I64, I64, I, I, I, I, I, I, I, F, P, P, SZ, P]),
+        "gfx906_fa_amd_scored_paged_attention": (I, [P, I, I64, I64, P, P, I64, I64, P, I64, P, P, P, I, F, P, P,
+                                                     I, I, I, I, I, I, I, I, F, P, I, I64, I64, P, SZ, P]),
+        "gfx906_fa_amd_qk_norm_rope_cache_write_kv": (I, [P, P, P, P, P, F, I, P, P, I, I64, I, I, I, P, P, P,
+                                                          I, I, I, I, I, I64, I64, I64, I64, I64, I64, I64, I64, P]),
+        "gfx906_fa_amd_read_rows": (I, [P, P, P, P, P, I, I64, I, I, I, I64, I64, I64, I64, I64, I64, I64, P]),
+        "gfx906_fa_amd_compact_draft_rows": (I, [P, P, P, P, I64, I, I64, I64, I64, P, I64, I, P, P, P, I64, I, P,
+                                                 I, I, I, I, P]),
         "gfx906_fa_amd_paged_attention_tiled": (I, [P, I, I64, I64, P, P, I, I64, I64, I64, I64, P, I64,
                                                     P, P, P, I, P, I64, I64, I, I, I, I, I, I, I, I,
                                                     F, P, I64, I64, P]),
@@ -592,6 +608,321 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     return out
 
 
+# ---------------------------------------------------------------------------
+# Scored and tree attention, norms with rotation, draft rows
+# ---------------------------------------------------------------------------
+MAX_TREE_NODES = 64
+
+
+def _on(dev: torch.device):
+    """The device current for a call's launches (no-op where it is already)."""
+    return nullcontext() if dev.index is None or torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _all_on(dev: torch.device, tensors, names: str) -> None:
+    for t, n in zip(tensors, names.split()):
+        if t is not None and t.device != dev:
+            _cuda(t, n)
+            raise RuntimeError(f"{n} must be on {dev}, got {t.device}")
+
+
+def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, max_query_len, max_seq_len, scale,
+            soft_cap, alibi_slopes, tree_mask, out, workspace, q_abs_offset, causal, out_dtype):
+    """scored_paged_attention and tree_attention: checks and the one call."""
+    if not query.is_cuda:
+        _cuda(query, "query")
+    dev = query.device
+    _all_on(dev, (key_cache, value_cache, block_table, seq_lens, query_start_loc, alibi_slopes, tree_mask, out,
+                  workspace, q_abs_offset),
+            "key_cache value_cache block_table seq_lens query_start_loc alibi_slopes tree_mask out workspace q_abs_offset")
+    if query.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("query must be fp16 or bf16")
+    qdt = _DT[query.dtype]
+    if query.dim() != 3 or query.shape[2] != 128:
+        raise RuntimeError("query must be [num_tokens, Hq, 128]")
+    T, Hq, D = query.shape
+    soft_cap = float(soft_cap)
+    if not 0.0 <= soft_cap < float("inf"):
+        raise RuntimeError(f"soft_cap must be 0 (none) or positive and finite, got {soft_cap}")
+    if alibi_slopes is not None:
+        if soft_cap > 0.0:
+            raise RuntimeError("soft_cap and alibi_slopes exclude each other")
+        if alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (Hq,) or not alibi_slopes.is_contiguous():
+            raise RuntimeError("alibi_slopes must be contiguous fp32 [Hq]")
+    if out_dtype is not None and out_dtype not in (query.dtype, torch.float32):
+        raise RuntimeError("out must be of the query dtype or fp32")
+    if T == 0:  # no query rows (an empty tensor's strides are arbitrary)
+        return out if out is not None else torch.empty((0, Hq, D), dtype=out_dtype or query.dtype, device=dev)
+    qts, qhs, qs = query.stride()
+    if qs != 1:
+        raise RuntimeError("query rows must be contiguous")
+    bs, Hkv, cbs, chs = _plane_info(key_cache, value_cache)
+    if Hkv == 0 or Hq % Hkv:
+        raise RuntimeError(f"heads_q={Hq} must be divisible by heads_kv={Hkv}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise RuntimeError("block_table must be int32 [num_seqs, max_blocks] with contiguous rows")
+    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+        raise RuntimeError("seq_lens must be contiguous int32")
+    if query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1 or not query_start_loc.is_contiguous():
+        raise RuntimeError("query_start_loc must be contiguous int32")
+    B = seq_lens.shape[0]
+    if block_table.shape[0] < B or query_start_loc.shape[0] < B + 1:
+        raise RuntimeError("block_table / query_start_loc shorter than seq_lens")
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 1 or tree_mask.shape[0] < T or not tree_mask.is_contiguous():
+            raise RuntimeError("tree_mask must be contiguous int64 [num_tokens]")
+        if max_query_len > MAX_TREE_NODES:
+            raise RuntimeError(f"a tree has at most {MAX_TREE_NODES} nodes (max_query_len {max_query_len})")
+    if q_abs_offset is not None:
+        _check(q_abs_offset.dtype == torch.int32 and q_abs_offset.is_contiguous()
+               and q_abs_offset.shape[0] >= B, "q_abs_offset must be int32 [B]")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=out_dtype or query.dtype, device=dev)
+    oshape, ostrides = out.shape, out.stride()
+    if out.dtype not in (query.dtype, torch.float32):
+        raise RuntimeError("out must be of the query dtype or fp32")
+    if len(oshape) != 3 or oshape[1] != Hq or oshape[2] != D or oshape[0] < T or ostrides[2] != 1:
+        raise RuntimeError("out must be [num_tokens, Hq, 128]")
+    if B == 0:
+        return out
+    L = _load()
+    with _on(dev):
+        need = L.gfx906_fa_amd_paged_attention_workspace_size(B, T, Hq, Hkv, D, max_query_len, max_seq_len)
+        if workspace is None or (workspace.nbytes < need and workspace.nbytes < plan_info(
+                B, T, Hq, Hkv, max_query_len, max_seq_len, D)["img_offset"]):
+            workspace = new_workspace(need, dev)
+        ws_ptr = workspace.data_ptr()
+        if ws_ptr % 256 or not workspace.is_contiguous():
+            raise RuntimeError("workspace must be contiguous and 256-byte aligned")
+        err = L.gfx906_fa_amd_scored_paged_attention(
+            query.data_ptr(), qdt, qts, qhs, key_cache.data_ptr(), value_cache.data_ptr(), cbs, chs,
+            block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), query_start_loc.data_ptr(),
+            _ptr(q_abs_offset), 1 if causal else 0, soft_cap, _ptr(alibi_slopes), _ptr(tree_mask), B, T, Hq, Hkv, D, bs,
+            int(max_query_len), int(max_seq_len), float(scale), out.data_ptr(), _DT[out.dtype], ostrides[0], ostrides[1],
+            ws_ptr, workspace.nbytes, _stream(dev))
+    if err:
+        _ok(err, "gfx906_fa_amd_scored_paged_attention")
+    return out
+
+
+def scored_paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                           block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
+                           max_query_len: int, max_seq_len: int, scale: float, soft_cap: float = 0.0,
+                           alibi_slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                           workspace: Optional[torch.Tensor] = None, q_abs_offset: Optional[torch.Tensor] = None,
+                           causal: bool = True, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``paged_attention`` with another score.  With s = scale * q.k:
+
+    ``soft_cap`` > 0: cap * tanh(s / cap).
+    ``alibi_slopes`` (fp32 [Hq]): s + slope[head] * (key position - row
+    position); row j of a sequence is at position seq_len - n_q + j, or at
+    q_abs_offset + j.  Rows of causal batches see no later key, so a positive
+    slope lowers the scores of far keys.
+
+    One of the two, or neither (plain attention).  query fp16 or bf16 [T, Hq,
+    128]; out of its dtype or fp32.  Lengths, workspace and errors as
+    ``paged_attention``: ``max_query_len`` / ``max_seq_len`` must bound the
+    device values.  A row that sees no key is 0; what the cache holds past a
+    sequence's keys does not matter, NaN and Inf included."""
+    return _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, max_query_len, max_seq_len,
+                   scale, soft_cap, alibi_slopes, None, out, workspace, q_abs_offset, causal, out_dtype)
+
+
+def tree_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, query_start_loc: torch.Tensor, tree_mask: torch.Tensor, max_query_len: int,
+                   max_seq_len: int, scale: float, soft_cap: float = 0.0, out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Verification of a tree of drafted tokens: the last n_q keys of each
+    sequence (already in the cache, ``seq_lens`` counts them) are the nodes of
+    its tree, node j the key of query row j.  Row j sees every key before them,
+    and the nodes i <= j whose bit i is set in ``tree_mask`` (int64 [T], at most
+    64 nodes; ``tree_masks`` makes them from parents).  Its own node is seen by
+    its own bit.  ``soft_cap`` and everything else as
+    ``scored_paged_attention``."""
+    if tree_mask is None:
+        raise RuntimeError("tree_mask is required")
+    return _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, max_query_len, max_seq_len,
+                   scale, soft_cap, None, tree_mask, out, workspace, None, True, out_dtype)
+
+
+def tree_masks(parents) -> torch.Tensor:
+    """Masks of ``tree_attention`` (int64, on the host) from the parents of each
+    node: one sequence's list, or a list of them, one per sequence.  A node's
+    parent comes before it; a root's is -1.  Bit i of a node's mask: node i is
+    it or one of its ancestors."""
+    trees = [list(parents)] if not len(parents) or isinstance(parents[0], int) else [list(t) for t in parents]
+    out = []
+    for tree in trees:
+        _check(len(tree) <= MAX_TREE_NODES, f"a tree has at most {MAX_TREE_NODES} nodes, got {len(tree)}")
+        masks = []
+        for i, p in enumerate(tree):
+            _check(-1 <= p < i, f"node {i}: its parent {p} must be -1 or an earlier node")
+            masks.append((masks[p] if p >= 0 else 0) | 1 << i)
+        out += [m - (1 << 64) if m >> 63 else m for m in masks]
+    return torch.tensor(out, dtype=torch.int64)
+
+
+def qk_norm_rope_and_cache_q8_kv(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                                 query_weight: torch.Tensor, key_weight: torch.Tensor, eps: float,
+                                 cos_sin_cache: torch.Tensor, is_neox: bool, slot_mapping: torch.Tensor,
+                                 key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                 rot_dim: Optional[int] = None) -> None:
+    """``rope_and_cache_q8_kv`` with an RMS norm of each head first: every head
+    row of query [T, Hq, 128] and key [T, Hkv, 128] becomes
+    x * rsqrt(mean(x^2) + eps) * weight (``query_weight`` / ``key_weight`` [128],
+    the model dtype), then its first rot_dim values are rotated, in place, in
+    fp32 and rounded once; the stored key and the value go to the cache as Q8_0
+    at slot_mapping (< 0 skips).  One launch.  Rows at positions outside
+    [0, max_position) are normed and not rotated."""
+    if not query.is_cuda:
+        _cuda(query, "query")
+    dev = query.device
+    _all_on(dev, (positions, key, value, query_weight, key_weight, cos_sin_cache, slot_mapping, key_cache, value_cache),
+            "positions key value query_weight key_weight cos_sin_cache slot_mapping key_cache value_cache")
+    dt = query.dtype
+    _check(dt in (torch.float16, torch.bfloat16) and key.dtype == dt and value.dtype == dt,
+           "query/key/value must share dtype fp16 or bf16")
+    _check(query.dim() == 3 and key.dim() == 3 and value.shape == key.shape and query.shape[0] == key.shape[0],
+           "query must be [T, Hq, D], key/value [T, Hkv, D]")
+    _check(positions.dtype == torch.int64 and positions.dim() == 1 and positions.shape[0] == query.shape[0],
+           "positions must be int64 [num_tokens]")
+    _check(slot_mapping.dtype == torch.int64 and slot_mapping.dim() == 1 and slot_mapping.shape[0] == query.shape[0],
+           "slot_mapping must be int64 [num_tokens]")
+    _check(cos_sin_cache.dtype in _DT and cos_sin_cache.dim() == 2 and cos_sin_cache.stride(1) == 1,
+           "cos_sin_cache must be [max_position, rot_dim] with contiguous rows")
+    T, Hq, D = query.shape
+    Hkv = key.shape[1]
+    _check(D == 128 and key.shape[2] == 128, "head_size must be 128")
+    for w, n in ((query_weight, "query_weight"), (key_weight, "key_weight")):
+        _check(w.dtype == dt and tuple(w.shape) == (128,) and w.is_contiguous(), f"{n} must be [128] of the query dtype")
+    _check(float(eps) >= 0.0, "eps must be >= 0")
+    if T == 0:  # nothing to do (an empty tensor's strides are arbitrary)
+        return
+    if query.stride(2) != 1 or key.stride(2) != 1 or value.stride(2) != 1:
+        raise RuntimeError("query, key and value rows must be contiguous")
+    rot = cos_sin_cache.shape[1] if rot_dim is None else int(rot_dim)
+    _check(rot <= cos_sin_cache.shape[1], f"rot_dim={rot} exceeds the {cos_sin_cache.shape[1]} columns of cos_sin_cache")
+    bs, Hc, cbs, chs = _plane_info(key_cache, value_cache)
+    if Hc != Hkv:
+        raise RuntimeError(f"cache Hkv mismatch: got {Hc} vs key Hkv={Hkv}")
+    if Hq % Hkv:
+        raise RuntimeError(f"heads_q={Hq} must be divisible by heads_kv={Hkv}")
+    pos = positions.contiguous()
+    sm = slot_mapping.contiguous()
+    with _on(dev):
+        err = _load().gfx906_fa_amd_qk_norm_rope_cache_write_kv(
+            _ptr(query), _ptr(key), _ptr(value), _ptr(query_weight), _ptr(key_weight), float(eps), _DT[dt], _ptr(pos),
+            _ptr(cos_sin_cache), _DT[cos_sin_cache.dtype], cos_sin_cache.stride(0), cos_sin_cache.shape[0], rot,
+            1 if is_neox else 0, _ptr(sm), _ptr(key_cache), _ptr(value_cache), T, Hq, Hkv, D, bs,
+            query.stride(0), query.stride(1), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+            cbs, chs, _stream(dev))
+    _ok(err, "gfx906_fa_amd_qk_norm_rope_cache_write_kv")
+
+
+def read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     dtype: torch.dtype = torch.float16, k_out: Optional[torch.Tensor] = None,
+                     v_out: Optional[torch.Tensor] = None):
+    """The reverse of ``reshape_and_cache_q8_kv``: the rows at slot_mapping
+    (int64 [T]) back as values, (k, v) [T, Hkv, 128] of ``dtype`` (fp16, bf16,
+    fp32), int8 * scale rounded once.  Slots outside the cache (< 0 too) give
+    zeros.  ``k_out`` / ``v_out`` are filled where given (that shape and dtype,
+    contiguous last dim, rows 16-byte aligned)."""
+    if not slot_mapping.is_cuda:
+        _cuda(slot_mapping, "slot_mapping")
+    dev = slot_mapping.device
+    _all_on(dev, (key_cache, value_cache, k_out, v_out), "key_cache value_cache k_out v_out")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1:
+        raise RuntimeError("slot_mapping must be int64 [num_tokens]")
+    odt = _DT.get(dtype)
+    if odt is None:
+        raise RuntimeError("dtype must be fp16, bf16 or fp32")
+    bs, Hkv, cbs, chs = _plane_info(key_cache, value_cache)
+    T = slot_mapping.shape[0]
+    outs = []
+    for o, n in ((k_out, "k_out"), (v_out, "v_out")):
+        if o is None:
+            o = torch.empty((T, Hkv, 128), dtype=dtype, device=dev)
+        elif o.shape != (T, Hkv, 128) or o.dtype != dtype or (T and o.stride(2) != 1):
+            raise RuntimeError(f"{n} must be [num_tokens, Hkv, 128] of dtype {dtype} with contiguous rows")
+        outs.append(o)
+    k, v = outs
+    if T == 0 or Hkv == 0:
+        return k, v
+    sm = slot_mapping.contiguous()
+    with _on(dev):
+        err = _load().gfx906_fa_amd_read_rows(
+            key_cache.data_ptr(), value_cache.data_ptr(), sm.data_ptr(), k.data_ptr(), v.data_ptr(), odt, T, Hkv, 128, bs,
+            key_cache.shape[0], cbs, chs, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _stream(dev))
+    if err:
+        _ok(err, "gfx906_fa_amd_read_rows")
+    return k, v
+
+
+def compact_draft_rows(kv_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
+                       accepted: torch.Tensor, num_accepted: torch.Tensor) -> None:
+    """Keeps the accepted draft tokens of a tree step: with n_q drafts in each
+    sequence's last rows (``seq_lens`` counts them, ``query_start_loc`` gives
+    n_q) and ctx = seq_len - n_q, the K and V rows at position
+    ctx + accepted[s, i] are copied to position ctx + i, for i below
+    num_accepted[s], in every kv-head and layer.  ``accepted`` int32 [B, A], A
+    <= 64, ``num_accepted`` int32 [B].  All rows of a sequence are read before
+    any is written.  Entries outside [0, n_q) are skipped, as are positions
+    outside the block table; rows past the kept ones stay as they were, and the
+    caller shortens the sequence to ctx + num_accepted.
+
+    ``kv_caches``: one stacked tensor, uint8 [layers, NB, 2, Hkv, bs/16*2176],
+    or a sequence of (key_cache, value_cache) planes, one pair per layer, of
+    one shape and one set of strides.  Sequences must not share draft pages."""
+    list_ptrs = (None, None)
+    if isinstance(kv_caches, torch.Tensor):
+        if kv_caches.dim() != 5 or kv_caches.shape[2] != 2 or kv_caches.dtype != torch.uint8:
+            raise RuntimeError("kv_caches must be uint8 [layers, num_blocks, 2, Hkv, block_size/16*2176]")
+        layers, lstride = kv_caches.shape[0], kv_caches.stride(0)
+        if layers == 0:
+            return
+        kc, vc = kv_caches[0, :, 0], kv_caches[0, :, 1]
+    else:
+        pairs = list(kv_caches)
+        layers, lstride = len(pairs), 0
+        if layers == 0:
+            return
+        kc, vc = pairs[0]
+        shape, strides, dev0 = kc.shape, kc.stride(), kc.device
+        for k, v in pairs:
+            for t in (k, v):
+                if t.shape != shape or t.stride() != strides or t.dtype != torch.uint8 or t.device != dev0:
+                    raise RuntimeError("every layer's planes must be uint8 of one shape, set of strides and device")
+        list_ptrs = tuple((ctypes.c_void_p * layers)(*(p[i].data_ptr() for p in pairs)) for i in range(2))
+    bs, Hkv, cbs, chs = _plane_info(kc, vc)
+    if not kc.is_cuda:
+        _cuda(kc, "kv_caches")
+    dev = kc.device
+    _all_on(dev, (block_table, seq_lens, query_start_loc, accepted, num_accepted),
+            "block_table seq_lens query_start_loc accepted num_accepted")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise RuntimeError("block_table must be int32 [num_seqs, max_blocks] with contiguous rows")
+    for t, n in ((seq_lens, "seq_lens"), (query_start_loc, "query_start_loc"), (num_accepted, "num_accepted")):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise RuntimeError(f"{n} must be contiguous int32")
+    B = seq_lens.shape[0]
+    if block_table.shape[0] < B or query_start_loc.shape[0] < B + 1 or num_accepted.shape[0] < B:
+        raise RuntimeError("block_table / query_start_loc / num_accepted shorter than seq_lens")
+    if accepted.dtype != torch.int32 or accepted.dim() != 2 or accepted.shape[0] < B or accepted.stride(1) != 1:
+        raise RuntimeError("accepted must be int32 [num_seqs, at most 64] with contiguous rows")
+    if accepted.shape[1] > MAX_TREE_NODES:
+        raise RuntimeError(f"accepted has at most {MAX_TREE_NODES} columns, got {accepted.shape[1]}")
+    if B == 0 or accepted.shape[1] == 0 or Hkv == 0:
+        return
+    with _on(dev):
+        err = _load().gfx906_fa_amd_compact_draft_rows(
+            list_ptrs[0], list_ptrs[1], kc.data_ptr(), vc.data_ptr(), lstride, layers, cbs, chs, kc.shape[0],
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+            query_start_loc.data_ptr(), accepted.data_ptr(), accepted.stride(0), accepted.shape[1],
+            num_accepted.data_ptr(), B, Hkv, 128, bs, _stream(dev))
+    if err:
+        _ok(err, "gfx906_fa_amd_compact_draft_rows")
+
+
 def _mask_args(mask: Optional[torch.Tensor], B: int, Sq: int, q_abs_offset):
     """fp16 additive mask [B, Sq, Skv_pad] (``extension/gfx906_fa.cpp:214-227``)
     -> (tensor, batch stride, row stride, columns) for the C entries."""
@@ -878,10 +1209,74 @@ def _register_torch_ops() -> None:
           slot_mapping=None):
         return None
 
+    @custom_op(f"{_NS}::scored_paged_attention", mutates_args=("workspace",))
+    def _scored_paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
+                                max_query_len: int, max_seq_len: int, scale: float, soft_cap: float,
+                                alibi_slopes: Optional[torch.Tensor], workspace: Optional[torch.Tensor],
+                                q_abs_offset: Optional[torch.Tensor] = None, causal: bool = True,
+                                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return scored_paged_attention(query, key_cache, value_cache, block_table, seq_lens, query_start_loc,
+                                      max_query_len, max_seq_len, scale, soft_cap, alibi_slopes, workspace=workspace,
+                                      q_abs_offset=q_abs_offset, causal=causal, out_dtype=out_dtype)
+
+    @_scored_paged_attention.register_fake
+    def _(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, max_query_len, max_seq_len, scale,
+          soft_cap, alibi_slopes, workspace, q_abs_offset=None, causal=True, out_dtype=None):
+        return query.new_empty(query.shape, dtype=out_dtype or query.dtype)
+
+    @custom_op(f"{_NS}::tree_attention", mutates_args=("workspace",))
+    def _tree_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                        block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
+                        tree_mask: torch.Tensor, max_query_len: int, max_seq_len: int, scale: float, soft_cap: float,
+                        workspace: Optional[torch.Tensor], out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        return tree_attention(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, tree_mask,
+                              max_query_len, max_seq_len, scale, soft_cap, workspace=workspace, out_dtype=out_dtype)
+
+    @_tree_attention.register_fake
+    def _(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, tree_mask, max_query_len, max_seq_len,
+          scale, soft_cap, workspace, out_dtype=None):
+        return query.new_empty(query.shape, dtype=out_dtype or query.dtype)
+
+    @custom_op(f"{_NS}::qk_norm_rope_and_cache_q8_kv", mutates_args=("query", "key", "key_cache", "value_cache"))
+    def _qk_norm_rope_and_cache_q8_kv(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
+                                      value: torch.Tensor, query_weight: torch.Tensor, key_weight: torch.Tensor,
+                                      eps: float, cos_sin_cache: torch.Tensor, is_neox: bool,
+                                      slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                      rot_dim: Optional[int] = None) -> None:
+        qk_norm_rope_and_cache_q8_kv(positions, query, key, value, query_weight, key_weight, eps, cos_sin_cache,
+                                     is_neox, slot_mapping, key_cache, value_cache, rot_dim)
+
+    @_qk_norm_rope_and_cache_q8_kv.register_fake
+    def _(positions, query, key, value, query_weight, key_weight, eps, cos_sin_cache, is_neox, slot_mapping, key_cache,
+          value_cache, rot_dim=None):
+        return None
+
+    @custom_op(f"{_NS}::read_cache_q8_kv", mutates_args=())
+    def _read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+        return read_cache_q8_kv(slot_mapping, key_cache, value_cache, dtype)
+
+    @_read_cache_q8_kv.register_fake
+    def _(slot_mapping, key_cache, value_cache, dtype):
+        shape = (slot_mapping.shape[0], key_cache.shape[1], 128)
+        return key_cache.new_empty(shape, dtype=dtype), key_cache.new_empty(shape, dtype=dtype)
+
+    @custom_op(f"{_NS}::compact_draft_rows", mutates_args=("kv_caches",))
+    def _compact_draft_rows(kv_caches: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                            query_start_loc: torch.Tensor, accepted: torch.Tensor, num_accepted: torch.Tensor) -> None:
+        compact_draft_rows(kv_caches, block_table, seq_lens, query_start_loc, accepted, num_accepted)
+
+    @_compact_draft_rows.register_fake
+    def _(kv_caches, block_table, seq_lens, query_start_loc, accepted, num_accepted):
+        return None
+
 
 TORCH_OPS = ("quantize_q8_0", "reshape_and_cache_q8", "gather_paged_kv_q8", "gather_paged_kv_q8_out",
              "forward", "forward_paged_direct", "reshape_and_cache_q8_kv", "rope_and_cache_q8_kv",
              "gather_paged_kv_q8q8", "paged_attention", "paged_attention_out")
+SCORED_TORCH_OPS = ("scored_paged_attention", "tree_attention", "qk_norm_rope_and_cache_q8_kv", "read_cache_q8_kv",
+                    "compact_draft_rows")
 
 _load()
 if not hasattr(torch.ops, _NS) or not hasattr(getattr(torch.ops, _NS), "paged_attention"):

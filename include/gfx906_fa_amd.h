@@ -456,6 +456,77 @@ hipError_t gfx906_fa_amd_paged_attention_padded(
     int batch, int seq_q, int num_heads, int num_kv_heads, int head_size, int block_size, int max_seq_len, float scale,
     float *out, void *workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* (11) Scored paged attention: (5) with another score.  With s = scale * q.k
+ *     soft_cap > 0:   cap * tanh(s / cap)
+ *     alibi_slopes:   s + slopes[head] * (key position - row position); fp32
+ *                     [num_heads], row j at position seq_len - n_q + j (or
+ *                     q_abs_offset + j)
+ *     tree_mask:      the sequence's last n_q keys are the nodes of a tree
+ *                     (node j: query row j), and row j sees every key before
+ *                     them and the nodes i <= j whose bit i is set in
+ *                     tree_mask[row], int64 [num_tokens] (its own node too
+ *                     only by its bit).  Causal, without q_abs_offset, n_q <=
+ *                     64.
+ *     soft_cap and tree_mask go together; alibi_slopes alone.  Without any of
+ *     them the call is (5).  query fp16 or bf16, out of its type or fp32.
+ *     Workspace and plan as (5).  A row that sees no key is 0.  K and V of
+ *     keys that no row sees, or that some row does not see, may hold anything;
+ *     a V block a row sees has to have a finite scale. */
+hipError_t gfx906_fa_amd_scored_paged_attention(
+    const void *q, int q_dtype, int64_t q_token_stride, int64_t q_head_stride,
+    const uint8_t *k_cache, const uint8_t *v_cache, int64_t cache_block_stride,
+    int64_t cache_head_stride, const int32_t *block_table, int64_t block_table_stride,
+    const int32_t *seq_lens, const int32_t *query_start_loc, const int32_t *q_abs_offset,
+    int causal, float soft_cap, const float *alibi_slopes, const int64_t *tree_mask,
+    int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int head_size,
+    int block_size, int max_query_len, int max_seq_len, float scale, void *out, int out_dtype,
+    int64_t out_token_stride, int64_t out_head_stride, void *workspace, size_t workspace_bytes,
+    hipStream_t stream);
+
+/* (12) (4b) with the RMS norm of each query and key head before the rotation:
+ *     y = x * rsqrt(mean(x^2) + eps) * weight over the 128 values of a head
+ *     (query_weight, key_weight: [128] of the model dtype, 16-byte aligned),
+ *     then the rotary pairs, in fp32 and rounded once to the model dtype as
+ *     query and key are stored in place.  The cache takes the stored key.
+ *     Positions outside [0, max_position) are normed and not rotated. */
+hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
+    void *query, void *key, const void *value, const void *query_weight, const void *key_weight,
+    float eps, int dtype, const int64_t *positions,
+    const void *cos_sin_cache, int cos_sin_dtype, int64_t cos_sin_stride, int max_position,
+    int rot_dim, int is_neox, const int64_t *slot_mapping, uint8_t *k_cache, uint8_t *v_cache,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size,
+    int64_t query_token_stride, int64_t query_head_stride, int64_t key_token_stride,
+    int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
+    int64_t cache_block_stride, int64_t cache_head_stride, hipStream_t stream);
+
+/* (13) Rows of the planar cache back as values: k_out / v_out
+ *     [num_rows][num_kv_heads][128] (fp32, fp16 or bf16; element strides,
+ *     multiples of 8, 16-byte aligned bases) receive int8 * scale of the rows
+ *     at slot_mapping (int64 [num_rows]), rounded once.  Slots outside the
+ *     cache of num_blocks pages (negative ones too) give zeros. */
+hipError_t gfx906_fa_amd_read_rows(
+    const uint8_t *k_cache, const uint8_t *v_cache, const int64_t *slot_mapping, void *k_out, void *v_out, int out_dtype,
+    int64_t num_rows, int num_kv_heads, int head_size, int block_size, int64_t num_blocks, int64_t cache_block_stride,
+    int64_t cache_head_stride, int64_t k_out_row_stride, int64_t k_out_head_stride, int64_t v_out_row_stride,
+    int64_t v_out_head_stride, hipStream_t stream);
+
+/* (14) Accepted draft tokens moved behind their context: with ctx = seq_lens[s]
+ *     - n_q (n_q from query_start_loc), row ctx + accepted[s][i] of K and V is
+ *     copied to row ctx + i, for i < min(num_accepted[s], accepted_cols, n_q),
+ *     every kv-head and layer; all rows of a sequence are read before any is
+ *     written.  accepted int32 [num_seqs][accepted_cols] (at most 64 columns),
+ *     num_accepted int32 [num_seqs].  Entries outside [0, n_q), positions
+ *     outside the block table and pages outside [0, num_blocks) are skipped.
+ *     The layers' planes: k_layers / v_layers (host arrays of num_layers device
+ *     pointers), or, with those NULL, k_cache / v_cache + layer * layer_stride
+ *     bytes.  All layers share the page strides (bytes) and the block table. */
+hipError_t gfx906_fa_amd_compact_draft_rows(
+    uint8_t *const *k_layers, uint8_t *const *v_layers, uint8_t *k_cache, uint8_t *v_cache, int64_t layer_stride,
+    int num_layers, int64_t cache_block_stride, int64_t cache_head_stride, int64_t num_blocks, const int32_t *block_table,
+    int64_t block_table_stride, int block_table_cols, const int32_t *seq_lens, const int32_t *query_start_loc,
+    const int32_t *accepted, int64_t accepted_stride, int accepted_cols, const int32_t *num_accepted, int num_seqs,
+    int num_kv_heads, int head_size, int block_size, hipStream_t stream);
+
 /* Measurement helper: streams `bytes` (a multiple of 16) from the 16-byte
  * aligned device buffer `src` with non-temporal 16-byte loads and writes one
  * XOR word per wave to `out` (at least gfx906_fa_amd_stream_read_words()

@@ -457,23 +457,51 @@ __device__ __forceinline__ void load_score_rows(const AttnParams &p, int h, int 
     }
 }
 
-// attend_subpage with the scored forms.  The scores are brought to log2 units
-// (y) before the mask and the maximum.  In a masked sub-page (one that some
-// row does not see in full) the V scales are made finite, as a hidden key's
-// P = 0 does not cancel an Inf or a NaN.
+// The operands of a sub-page for the scored forms: the K scales of the four
+// tokens 4g .. 4g + 3 whose scores the lane holds, four blocks each, instead of
+// those of its own token.
+struct SubPageS {
+    u32x4 kq[2], ks[2], vq[2], vs[2];
+};
+
+template <bool NT>
+__device__ __forceinline__ void load_subpage(SubPageS &sp, const uint8_t *kb, const uint8_t *vb,
+                                             const LaneOffsets &lo) {
+    const u32x4 *k0 = reinterpret_cast<const u32x4 *>(kb + lo.kq);
+    const u32x4 *ks = reinterpret_cast<const u32x4 *>(kb + lo.vs);  // (the offset of tokens 4g .. in either table)
+    const u32x4 *v0 = reinterpret_cast<const u32x4 *>(vb + lo.vq);
+    const u32x4 *vs = reinterpret_cast<const u32x4 *>(vb + lo.vs);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (NT) {
+            sp.kq[i] = __builtin_nontemporal_load(k0 + 64 * i);
+            sp.vq[i] = __builtin_nontemporal_load(v0 + 64 * i);
+        } else {
+            sp.kq[i] = k0[64 * i];
+            sp.vq[i] = v0[64 * i];
+        }
+        sp.ks[i] = ks[i];
+        sp.vs[i] = vs[i];
+    }
+}
+
+// attend_subpage with the scored forms.  K's int8 values enter the MFMA as they
+// are, and the scores of its four blocks are scaled and added in fp32 (16
+// mixed-precision multiply-adds a row group, the count of packed products that
+// K^ = fp16(q * d_k) takes for one row group); p * d_v is formed in fp32 and
+// rounded to fp16 once.  An fp16 output is then within 1.4 times its own
+// rounding of the 64-bit one (1.9 with K^ and P rounded on their way).
+// The scores are brought to log2 units (y) before the mask and the maximum.
+// In a masked sub-page (one that some row does not see in full) the V scales
+// are made finite, as a hidden key's P = 0 does not cancel an Inf or a NaN.
 template <int NRG, int SC>
-__device__ __forceinline__ void attend_subpage_scored(WaveAcc<NRG> &acc, const SubPage &sp,
+__device__ __forceinline__ void attend_subpage_scored(WaveAcc<NRG> &acc, const SubPageS &sp,
                                                       const half8_t (&qf)[NRG][4], int tok0, int kv_end,
                                                       const int (&lim)[NRG], const ScoreRows<NRG, SC> &sr, float c,
                                                       int g, bool mask) {
     half8_t ka[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const uint32_t sw = sp.ks[b >> 1];
-        const half_t d = __builtin_bit_cast(half2_t, sw)[b & 1];
-        const half8_t dd = {d, d, d, d, d, d, d, d};
-        ka[b] = i8x8_to_half8(dw(sp.kq, 2 * b), dw(sp.kq, 2 * b + 1)) * dd;
-    }
+    for (int b = 0; b < 4; ++b) ka[b] = i8x8_to_half8(dw(sp.kq, 2 * b), dw(sp.kq, 2 * b + 1));
     half2_t vs[8];
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
@@ -486,9 +514,16 @@ __device__ __forceinline__ void attend_subpage_scored(WaveAcc<NRG> &acc, const S
     }
 #pragma unroll
     for (int rg = 0; rg < NRG; ++rg) {
-        float4_t sacc = mfma16(ka[0], qf[rg][0], float4_t{0.f, 0.f, 0.f, 0.f});
+        float4_t sb[4], sacc;
 #pragma unroll
-        for (int b = 1; b < 4; ++b) sacc = mfma16(ka[b], qf[rg][b], sacc);
+        for (int b = 0; b < 4; ++b) sb[b] = mfma16(ka[b], qf[rg][b], float4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w0 = dw(sp.ks, 2 * i), w1 = dw(sp.ks, 2 * i + 1);
+            const half2_t d0 = __builtin_bit_cast(half2_t, w0), d1 = __builtin_bit_cast(half2_t, w1);
+            sacc[i] = fmaf(sb[3][i], (float)d1[1],
+                           fmaf(sb[2][i], (float)d1[0], fmaf(sb[1][i], (float)d0[1], sb[0][i] * (float)d0[0])));
+        }
         float y[4];
         const float kb = SC == SC_BIAS ? (float)(tok0 + 4 * g - sr.pos[rg]) * sr.slope[rg] : 0.0f;
 #pragma unroll
@@ -522,15 +557,11 @@ __device__ __forceinline__ void attend_subpage_scored(WaveAcc<NRG> &acc, const S
 #pragma unroll
         for (int i = 0; i < 4; ++i) pr[i] = __builtin_amdgcn_exp2f(y[i] - nm);
         acc.l[rg] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-        const half2_t p01 = {(half_t)pr[0], (half_t)pr[1]};
-        const half2_t p23 = {(half_t)pr[2], (half_t)pr[3]};
         half4_t pb[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const half2_t a = p01 * vs[2 * b];
-            const half2_t c2 = p23 * vs[2 * b + 1];
-            pb[b] = half4_t{a[0], a[1], c2[0], c2[1]};
-        }
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pb[b][i] = (half_t)fmaf(pr[i], (float)vs[2 * b + (i >> 1)][i & 1], 0.0f);
 #pragma unroll
         for (int mm = 0; mm < 8; ++mm) {
             half2_t lo, hi;
@@ -608,7 +639,8 @@ __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams
     const float c = p.scale_log2e;
     const LaneOffsets lo = lane_offsets(i16, g);
 
-    auto fetch = [&](SubPage &sp, int j) {
+    using SP = std::conditional_t<SC == SC_NONE, SubPage, SubPageS>;
+    auto fetch = [&](SP &sp, int j) {
         if (j < nsub) {
             if ((j >> 6) != chunk) {  // advance the page-id window (uniform)
                 chunk = j >> 6;
@@ -623,7 +655,7 @@ __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams
         }
     };
     // ring of DEPTH sub-page buffers: DEPTH-1 sub-pages in flight while one computes
-    SubPage buf[DEPTH];
+    SP buf[DEPTH];
 #pragma unroll
     for (int u = 0; u < DEPTH - 1; ++u) fetch(buf[u], u);
     for (int base = 0; base < nsub; base += DEPTH) {
@@ -781,10 +813,15 @@ __device__ __forceinline__ void stream_range_lds(WaveAcc<NRG> &acc, const AttnPa
                 fetch(j + DEPTH - 1, (u + DEPTH - 1) % DEPTH);
                 landed(j);
                 const uint8_t *sb = ring + u * DEC_RING_SLOT;
-                SubPage sp;
+                std::conditional_t<SC == SC_NONE, SubPage, SubPageS> sp;
                 sp.kq[0] = *reinterpret_cast<const u32x4 *>(sb + lo.kq);
                 sp.kq[1] = *reinterpret_cast<const u32x4 *>(sb + lo.kq + 1024);
-                sp.ks = *reinterpret_cast<const u32x2 *>(sb + lo.ks);
+                if constexpr (SC == SC_NONE) {
+                    sp.ks = *reinterpret_cast<const u32x2 *>(sb + lo.ks);
+                } else {
+                    sp.ks[0] = *reinterpret_cast<const u32x4 *>(sb + lo.vs);
+                    sp.ks[1] = *reinterpret_cast<const u32x4 *>(sb + lo.vs + 16);
+                }
                 sp.vq[0] = *reinterpret_cast<const u32x4 *>(sb + SUBPAGE_BYTES + lo.vq);
                 sp.vq[1] = *reinterpret_cast<const u32x4 *>(sb + SUBPAGE_BYTES + lo.vq + 1024);
                 sp.vs[0] = *reinterpret_cast<const u32x4 *>(sb + SUBPAGE_BYTES + lo.vs);

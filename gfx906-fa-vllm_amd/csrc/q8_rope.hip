@@ -394,7 +394,12 @@ __device__ __forceinline__ void load_cs_f32(const void *row, int col, float (&v)
     for (int e = 0; e < N; e += 2) load2_as_f32<CSDT>(row, col + e, v[e], v[e + 1]);
 }
 
-template <int DT, int CSDT, bool NEOX>
+#ifndef GFA_NORM_FEW_WAVES
+#define GFA_NORM_FEW_WAVES 2048
+#endif
+constexpr int NORM_FEW_WAVES = GFA_NORM_FEW_WAVES;
+
+template <int DT, int CSDT, bool NEOX, int ITERS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q8_norm_rope_cache_write_kernel(NormArgs n) {
     const RopeArgs &a = n.r;
     const int64_t wave = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -403,11 +408,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
     const int d0 = 8 * i;
     const int64_t t = wave / a.nchunk;
     if (t >= a.num_tokens) return;  // uniform over the wave
-    const int c0 = 4 * ROPE_ITERS * (int)(wave - t * a.nchunk);
+    const int c0 = 4 * ITERS * (int)(wave - t * a.nchunk);
     const int R = a.Hq + a.Hkv;
-    u32x4_t xw[ROPE_ITERS], vw[ROPE_ITERS];
+    u32x4_t xw[ITERS], vw[ITERS];
 #pragma unroll
-    for (int it = 0; it < ROPE_ITERS; ++it) {
+    for (int it = 0; it < ITERS; ++it) {
         xw[it] = u32x4_t{0, 0, 0, 0};
         vw[it] = u32x4_t{0, 0, 0, 0};
         const int row = c0 + 4 * it + g;
@@ -446,7 +451,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
     load8_f32<DT>(n.wq, d0, wq);
     load8_f32<DT>(n.wk, d0, wk);
 #pragma unroll
-    for (int it = 0; it < ROPE_ITERS; ++it) {
+    for (int it = 0; it < ITERS; ++it) {
         if (c0 + 4 * it >= R) break;  // uniform: no row of this iteration exists
         const int row = c0 + 4 * it + g;
         const bool active = row < R;  // the same for the 16 lanes of a row
@@ -501,9 +506,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
 }
 
 template <int DT, int CSDT>
-void launch_norm_rope(const NormArgs &a, bool neox, unsigned grid, hipStream_t stream) {
-    if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true><<<grid, 256, 0, stream>>>(a);
-    else q8_norm_rope_cache_write_kernel<DT, CSDT, false><<<grid, 256, 0, stream>>>(a);
+void launch_norm_rope(const NormArgs &a, bool neox, hipStream_t stream) {
+    NormArgs n = a;
+    const int rows = a.r.Hq + a.r.Hkv;
+    // few tokens: 8 rows a wave instead of 32, so that more waves share them
+    const bool few = a.r.num_tokens * ((rows + 31) / 32) < NORM_FEW_WAVES;
+    const int per = 4 * (few ? 2 : ROPE_ITERS);
+    n.r.nchunk = (rows + per - 1) / per;
+    const unsigned grid = (unsigned)((a.r.num_tokens * n.r.nchunk + 3) / 4);
+    if (few) {
+        if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true, 2><<<grid, 256, 0, stream>>>(n);
+        else q8_norm_rope_cache_write_kernel<DT, CSDT, false, 2><<<grid, 256, 0, stream>>>(n);
+    } else {
+        if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true, ROPE_ITERS><<<grid, 256, 0, stream>>>(n);
+        else q8_norm_rope_cache_write_kernel<DT, CSDT, false, ROPE_ITERS><<<grid, 256, 0, stream>>>(n);
+    }
 }
 
 // Checks an entry's arguments and fills in the kernel's; grid 0: nothing to do.
@@ -647,9 +664,9 @@ extern "C" hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
     const bool neox = is_neox != 0;
 #define GFA_NORM_CS(DT)                                                     \
     switch (cos_sin_dtype) {                                                \
-        case GFA_DTYPE_F32: launch_norm_rope<DT, GFA_DTYPE_F32>(a, neox, grid, stream); break; \
-        case GFA_DTYPE_F16: launch_norm_rope<DT, GFA_DTYPE_F16>(a, neox, grid, stream); break; \
-        default: launch_norm_rope<DT, GFA_DTYPE_BF16>(a, neox, grid, stream); break;           \
+        case GFA_DTYPE_F32: launch_norm_rope<DT, GFA_DTYPE_F32>(a, neox, stream); break; \
+        case GFA_DTYPE_F16: launch_norm_rope<DT, GFA_DTYPE_F16>(a, neox, stream); break; \
+        default: launch_norm_rope<DT, GFA_DTYPE_BF16>(a, neox, stream); break;           \
     }
     if (dtype == GFA_DTYPE_F16) {
         GFA_NORM_CS(GFA_DTYPE_F16)

@@ -14,7 +14,12 @@ using namespace gfa;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Rows back as values: wave per (row, kv-head), two values per lane.
+// Rows back as values.  A wave takes 16 consecutive entries of slot_mapping for
+// one kv-head.  Where they are a sub-page in order (a prompt's rows), it reads
+// the sub-page's 2 x 2176 bytes once, 16 bytes a lane; a lane then holds runs of
+// 8 values of a K row, and of a V chunk 4 values of 4 tokens, which go through
+// LDS to become rows.  Otherwise 16 lanes take a row, 8 values each: one 8-byte
+// K load and 8 dwords of V (each with a byte of the row), four rows at a time.
 struct ReadArgs {
     const uint8_t *kc, *vc;
     const int64_t *slot;
@@ -25,142 +30,319 @@ struct ReadArgs {
 };
 
 template <int ODT>
-__device__ __forceinline__ void store2(void *out, int64_t i, float a, float b) {
+__device__ __forceinline__ uint16_t out16(float v) {
+    if constexpr (ODT == GFA_DTYPE_F16) return f32_to_half_bits(v);
+    else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+// 8 values at a 16-byte aligned element offset
+template <int ODT>
+__device__ __forceinline__ void store8(void *out, int64_t i, const float (&v)[8]) {
     if constexpr (ODT == GFA_DTYPE_F32) {
-        *reinterpret_cast<float2 *>(static_cast<float *>(out) + i) = make_float2(a, b);
-    } else if constexpr (ODT == GFA_DTYPE_F16) {
-        half2_t h = {(half_t)a, (half_t)b};
-        *reinterpret_cast<half2_t *>(static_cast<uint16_t *>(out) + i) = h;
+        float4_t *p = reinterpret_cast<float4_t *>(static_cast<float *>(out) + i);
+        p[0] = float4_t{v[0], v[1], v[2], v[3]};
+        p[1] = float4_t{v[4], v[5], v[6], v[7]};
     } else {
-        const uint32_t lo = __builtin_bit_cast(uint16_t, (__bf16)a), hi = __builtin_bit_cast(uint16_t, (__bf16)b);
-        *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(out) + i) = lo | hi << 16;
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = out16<ODT>(v[2 * e]) | (uint32_t)out16<ODT>(v[2 * e + 1]) << 16;
+        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(out) + i) = w;
     }
 }
 
+__device__ __forceinline__ float byte_f32(uint32_t w, int e) { return (float)(int8_t)(w >> (8 * e)); }
+
+constexpr int RR_PITCH = 132;  // floats of a V row in LDS: rows of a quad of tokens start 4 banks apart
+
 template <int ODT>
 __global__ __launch_bounds__(256) void read_rows_kernel(ReadArgs a) {
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int64_t t = w / a.Hkv;
-    if (t >= a.num_rows) return;
-    const int h = (int)(w - t * a.Hkv);
-    const int64_t slot = a.slot[t];
-    const int d = 2 * lane;
-    float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-    if (slot >= 0 && slot < a.num_slots) {
-        const int64_t page = slot / a.block_size;
-        const int off = (int)(slot - page * a.block_size);
+    __shared__ float sm[4][16][RR_PITCH];
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t w = (int64_t)blockIdx.x * 4 + wv;
+    const int64_t t0 = w / a.Hkv * 16;
+    if (t0 >= a.num_rows) return;  // uniform over the wave
+    const int h = (int)(w - t0 / 16 * a.Hkv);
+    const int n = (int)min((int64_t)16, a.num_rows - t0);
+    const int i = lane & 15, g = lane >> 4;
+    const int64_t mine = i < n ? a.slot[t0 + i] : -1;
+    const int64_t first = ((int64_t)__builtin_amdgcn_readfirstlane((int)(mine >> 32)) << 32) |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((int)mine);
+    if (n == 16 && first >= 0 && (first & 15) == 0 && first + 15 < a.num_slots &&
+        __builtin_amdgcn_ballot_w64(mine != first + i) == 0) {  // uniform
+        const int64_t page = first / a.block_size;
+        const int off = (int)(first - page * a.block_size);
         const int64_t sub = page * a.cbs + (int64_t)h * a.chs + (int64_t)(off >> 4) * SUBPAGE_BYTES;
         const uint8_t *ks = a.kc + sub, *vs = a.vc + sub;
-        const int tt = off & 15, b = d >> 5;
-        const int kp = (b >> 1) * 1024 + (4 * tt + ((d >> 3) & 3)) * 16 + (b & 1) * 8 + (d & 7);
-        const int vp = (d >> 6) * 1024 + (tt >> 2) * 256 + (d & 15) * 16 + ((d >> 4) & 3) * 4 + (tt & 3);
-        const float dk = half_bits_to_f32(*reinterpret_cast<const uint16_t *>(ks + SCALE_OFF + (4 * tt + b) * 2));
-        const float dv = half_bits_to_f32(
-            *reinterpret_cast<const uint16_t *>(vs + SCALE_OFF + ((tt >> 2) * 4 + b) * 8 + (tt & 3) * 2));
-        const uint16_t kq = *reinterpret_cast<const uint16_t *>(ks + kp);
-        k0 = (float)(int8_t)(kq & 0xFF) * dk;
-        k1 = (float)(int8_t)(kq >> 8) * dk;
-        v0 = (float)(int8_t)vs[vp] * dv;
-        v1 = (float)(int8_t)vs[vp + 16] * dv;
+        // K: lane 4 t + q holds values 64 c + 32 b + 8 q .. of token t in dwords 2 b, 2 b + 1 of chunk c
+        const u32x4 k0 = *reinterpret_cast<const u32x4 *>(ks + 16 * lane);
+        const u32x4 k1 = *reinterpret_cast<const u32x4 *>(ks + 1024 + 16 * lane);
+        // V: lane 16 u + e holds values 64 c + 16 m + e of tokens 4 u .. in dword m of chunk c
+        const u32x4 v0 = *reinterpret_cast<const u32x4 *>(vs + 16 * lane);
+        const u32x4 v1 = *reinterpret_cast<const u32x4 *>(vs + 1024 + 16 * lane);
+        const u32x2 kd = *reinterpret_cast<const u32x2 *>(ks + SCALE_OFF + 8 * (lane >> 2));
+        const u32x4 d0 = *reinterpret_cast<const u32x4 *>(vs + SCALE_OFF + 32 * g);
+        const u32x4 d1 = *reinterpret_cast<const u32x4 *>(vs + SCALE_OFF + 32 * g + 16);
+        const int t = lane >> 2;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const u32x4 kq = c ? k1 : k0;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float d = half_bits_to_f32(b ? kd[c] >> 16 : kd[c] & 0xFFFFu);
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = byte_f32(kq[2 * b + (e >> 2)], e & 3) * d;
+                store8<ODT>(a.ko, (t0 + t) * a.kts + (int64_t)h * a.khs + 64 * c + 32 * b + 8 * (lane & 3), x);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const u32x4 vq = c ? v1 : v0, vd = c ? d1 : d0;
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // token 4 g + e: scale of block 2 c + m / 2
+                    const uint32_t dw = vd[2 * (m >> 1) + (e >> 1)];
+                    const float d = half_bits_to_f32(e & 1 ? dw >> 16 : dw & 0xFFFFu);
+                    sm[wv][4 * g + e][64 * c + 16 * m + i] = byte_f32(vq[m], e) * d;
+                }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // one wave's LDS instructions complete in order
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float4_t *row = reinterpret_cast<const float4_t *>(&sm[wv][4 * r + g][8 * i]);
+            const float4_t p = row[0], q = row[1];
+            const float x[8] = {p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
+            store8<ODT>(a.vo, (t0 + 4 * r + g) * a.vts + (int64_t)h * a.vhs + 8 * i, x);
+        }
+        return;
     }
-    store2<ODT>(a.ko, t * a.kts + (int64_t)h * a.khs + d, k0, k1);
-    store2<ODT>(a.vo, t * a.vts + (int64_t)h * a.vhs + d, v0, v1);
+    // rows one by one: lane i of 16 takes values 8 i .. of entry 4 r + g
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int at = 4 * r + g;
+        if (4 * r >= n) break;  // uniform
+        const int64_t slot = ((int64_t)__shfl((int)(mine >> 32), at) << 32) | (uint32_t)__shfl((int)mine, at);
+        float k[8] = {}, v[8] = {};
+        if (slot >= 0 && slot < a.num_slots) {
+            const int64_t page = slot / a.block_size;
+            const int off = (int)(slot - page * a.block_size);
+            const int64_t sub = page * a.cbs + (int64_t)h * a.chs + (int64_t)(off >> 4) * SUBPAGE_BYTES;
+            const uint8_t *ks = a.kc + sub, *vs = a.vc + sub;
+            const int tt = off & 15, b = i >> 2, m = i >> 1;
+            const u32x2 kq = *reinterpret_cast<const u32x2 *>(ks + (b >> 1) * 1024 + (4 * tt + (i & 3)) * 16 + (b & 1) * 8);
+            const uint8_t *vp = vs + (m >> 2) * 1024 + (tt >> 2) * 256 + (i & 1) * 128 + (m & 3) * 4;
+            uint32_t vq[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) vq[e] = *reinterpret_cast<const uint32_t *>(vp + 16 * e);
+            const float dk = half_bits_to_f32(*reinterpret_cast<const uint16_t *>(ks + SCALE_OFF + (4 * tt + b) * 2));
+            const float dv = half_bits_to_f32(
+                *reinterpret_cast<const uint16_t *>(vs + SCALE_OFF + ((tt >> 2) * 4 + b) * 8 + (tt & 3) * 2));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                k[e] = byte_f32(kq[e >> 2], e & 3) * dk;
+                v[e] = byte_f32(vq[e], tt & 3) * dv;
+            }
+        }
+        if (at < n) {
+            store8<ODT>(a.ko, (t0 + at) * a.kts + (int64_t)h * a.khs + 8 * i, k);
+            store8<ODT>(a.vo, (t0 + at) * a.vts + (int64_t)h * a.vhs + 8 * i, v);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
 // Accepted draft rows: sequence s keeps draft tokens accepted[s][0 .. n-1] of
-// its n_q; row (context + accepted[s][i]) moves to row (context + i).  Every
-// row is read before any is written (a row may be one's source and another's
-// target), so one workgroup moves all rows of a (layer, sequence, kv-head,
-// plane), through LDS.
+// its n_q; row (context + accepted[s][i]) moves to row (context + i), as if
+// every row were read before any is written.  Where the rows lie is the same
+// for every layer and head: a workgroup works that out once, and its four
+// waves then take (layer, kv-head) pairs of the sequence, K and V.
+//
+// K rows are whole pieces of 16 and 8 bytes.  Of a V row every 16-byte chunk
+// holds one byte in four, so V moves by quads of target tokens: a lane loads the
+// target's chunk and those of up to four source rows, merges their bytes and
+// stores the chunk whole (byte stores left the memory with partial lines: 60
+// layers x 32 sequences 34 us, ? us this way).  A path's nodes
+// ascend (a node comes after its parent), so that no row is the target of an
+// earlier one, and a wave moves rows and quads in order, all loads of a step
+// before its stores.  In any other order all rows go through LDS first.
 constexpr int MAX_DRAFT = 64;
 constexpr int LAYERS = 64;  // layers of one launch, given one by one
+#ifndef GFA_CR_WAVES
+#define GFA_CR_WAVES 8192
+#endif
+constexpr int CR_WAVES = GFA_CR_WAVES;
+constexpr int MAX_QUADS = MAX_DRAFT / 4 + 1;
 
 struct CompactArgs {
     const int32_t *bt, *seq_lens, *qsl, *accepted, *count;
     int64_t bt_stride, acc_stride, cbs, chs, layer_stride, num_blocks;
-    int bt_cols, acc_cols, Hkv, block_size, list;
+    int bt_cols, acc_cols, Hkv, block_size, layers, list;
     uint8_t *k[LAYERS], *v[LAYERS];  // list: each layer's planes; else k[0], v[0] + layer * layer_stride
 };
 
-// byte offset of position pos of sequence s in a plane (its sub-page), or -1
-__device__ __forceinline__ int64_t sub_of(const CompactArgs &a, int s, int h, int64_t pos) {
+// byte offset of position pos of sequence s in a plane (its sub-page, kv-head 0), or -1
+__device__ __forceinline__ int64_t sub_of(const CompactArgs &a, int s, int64_t pos) {
     if (pos < 0) return -1;
     const int64_t col = pos / a.block_size;
     if (col >= a.bt_cols) return -1;
     const int64_t page = a.bt[(int64_t)s * a.bt_stride + col];
     if (page < 0 || page >= a.num_blocks) return -1;
     const int off = (int)(pos - col * a.block_size);
-    return page * a.cbs + (int64_t)h * a.chs + (int64_t)(off >> 4) * SUBPAGE_BYTES;
+    return page * a.cbs + (int64_t)(off >> 4) * SUBPAGE_BYTES;
 }
 
-__global__ __launch_bounds__(64) void compact_rows_kernel(CompactArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t rows[];  // [acc_cols][144]: 128 values, 8 bytes of scales
-    constexpr int PITCH = 144;
+constexpr int CR_PIECES = 8 + 1 + 32 + 2;   // K ints, K scales, V chunks, V scales
+constexpr int CR_QUAD = 32 + 2;             // V chunks and scale chunks of a quad of tokens
+
+// Byte offset in its plane's sub-page of piece c of token t, 16-byte aligned.
+__device__ __forceinline__ int piece_off(int c, int t) {
+    if (c < 8) return (c >> 2) * 1024 + 64 * t + (c & 3) * 16;
+    if (c == 8) return SCALE_OFF + (t >> 1) * 16;
+    if (c < 41) return ((c - 9) >> 4) * 1024 + (t >> 2) * 256 + ((c - 9) & 15) * 16;
+    return SCALE_OFF + (t >> 2) * 32 + (c - 41) * 16;
+}
+
+// Stores what piece c holds of token ts at token td of the sub-page p.
+__device__ __forceinline__ void piece_store(uint8_t *p, int c, int ts, int td, u32x4 x) {
+    uint8_t *const at = p + piece_off(c, td);
+    if (c < 8) {
+        *reinterpret_cast<u32x4 *>(at) = x;
+    } else if (c == 8) {
+        *reinterpret_cast<u32x2 *>(at + 8 * (td & 1)) = ts & 1 ? u32x2{x[2], x[3]} : u32x2{x[0], x[1]};
+    } else if (c < 41) {  // byte ts % 4 of each dword
+#pragma unroll
+        for (int e = 0; e < 4; ++e) at[4 * e + (td & 3)] = (uint8_t)(x[e] >> (8 * (ts & 3)));
+    } else {  // two blocks, four tokens' scales each
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const uint32_t w = ts & 2 ? x[2 * b + 1] : x[2 * b];
+            *reinterpret_cast<uint16_t *>(at + 8 * b + 2 * (td & 3)) = (uint16_t)(ts & 1 ? w >> 16 : w);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void compact_rows_kernel(CompactArgs a) {
+    extern __shared__ __attribute__((aligned(16))) u32x4 rows[];  // out of order: [acc_cols][CR_PIECES]
     __shared__ int64_t s_src[MAX_DRAFT], s_dst[MAX_DRAFT];
-    __shared__ int s_st[MAX_DRAFT], s_dt[MAX_DRAFT];
-    const int lane = threadIdx.x;
-    const int s = blockIdx.x / a.Hkv, h = blockIdx.x - s * a.Hkv;
-    const bool isv = blockIdx.y & 1;
-    const int layer = blockIdx.z;
-    uint8_t *const base = a.list ? (isv ? a.v[layer] : a.k[layer]) : (isv ? a.v[0] : a.k[0]) + layer * a.layer_stride;
-    const int nq = a.qsl[s + 1] - a.qsl[s];
-    const int n = min(min(a.count[s], a.acc_cols), MAX_DRAFT);
-    const int64_t ctx = (int64_t)a.seq_lens[s] - nq;
-    if (lane < n) {
-        const int from = a.accepted[(int64_t)s * a.acc_stride + lane];
-        const bool ok = from >= 0 && from < nq && lane < nq && from != lane;
-        const int64_t src = ok ? sub_of(a, s, h, ctx + from) : -1, dst = ok ? sub_of(a, s, h, ctx + lane) : -1;
-        s_src[lane] = dst < 0 ? -1 : src;
-        s_dst[lane] = dst;
-        s_st[lane] = (int)((ctx + from) % 16);  // (block sizes are multiples of 16)
-        s_dt[lane] = (int)((ctx + lane) % 16);
+    __shared__ int s_tok[MAX_DRAFT];  // token in the sub-page: source, target << 8
+    __shared__ int64_t s_quad[MAX_QUADS];  // target quads with a row: sub-page, and its quad in it in the low bits
+    __shared__ int s_row[MAX_QUADS][4];    // the row that each of its tokens takes, or -1
+    __shared__ int s_n, s_nquad, s_ascending;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int s = blockIdx.x;
+    if (wv == 0) {
+        // (loaded together: the entries past the count are not used)
+        const int entry = lane < a.acc_cols ? a.accepted[(int64_t)s * a.acc_stride + lane] : -1;
+        const int nq = a.qsl[s + 1] - a.qsl[s];
+        const int n = min(min(a.count[s], a.acc_cols), min(nq, MAX_DRAFT));
+        const int64_t ctx = (int64_t)a.seq_lens[s] - nq;
+        const int from = lane < n ? entry : -1;
+        const bool moves = from >= 0 && from < nq && from != lane;
+        const int64_t src = moves ? sub_of(a, s, ctx + from) : -1, dst = moves ? sub_of(a, s, ctx + lane) : -1;
+        const uint64_t ok = __builtin_amdgcn_ballot_w64(src >= 0 && dst >= 0);
+        // quads of targets: lane i is token (ctx + i) & 3 of one; a quad is led by its first lane that moves
+        const int tok = (int)((ctx + lane) & 3);
+        const int lead = lane - tok;  // the quad's token 0 (before lane 0 in the first quad)
+        const uint64_t quad_ok = (lead >= 0 ? ok >> lead : ok << -lead) & 15;  // bit w: token w of the quad moves
+        const bool leads = (ok >> lane & 1) && (quad_ok & ((1u << tok) - 1)) == 0;
+        const uint64_t leaders = __builtin_amdgcn_ballot_w64(leads);
+        if (leads) {
+            const int q = __builtin_popcountll(leaders & ((1ull << lane) - 1));
+            s_quad[q] = dst | (int)((ctx + lane) >> 2 & 3);
+            for (int w = 0; w < 4; ++w)
+                s_row[q][w] = quad_ok >> w & 1 ? __builtin_popcountll(ok & ((1ull << (lead + w)) - 1)) : -1;
+        }
+        if (src >= 0 && dst >= 0) {
+            const int at = __builtin_popcountll(ok & ((1ull << lane) - 1));
+            s_src[at] = src;
+            s_dst[at] = dst;
+            s_tok[at] = (int)((ctx + from) & 15) | (int)((ctx + lane) & 15) << 8;  // (block sizes are multiples of 16)
+        }
+        // no row is read after an earlier one was written over it where every
+        // row moves down: its source is behind all targets up to its own
+        const bool down = __builtin_amdgcn_ballot_w64(src >= 0 && dst >= 0 && from < lane) == 0;
+        if (lane == 0) {
+            s_n = __builtin_popcountll(ok);
+            s_nquad = __builtin_popcountll(leaders);
+            s_ascending = down;
+        }
     }
     __syncthreads();
-    // items of a row: 0..31 values (K: dword i of the row; V: the row's bytes of
-    // the 16-byte chunk a = i / 16, e = i % 16), 32..35 one scale each
-    for (int it = lane; it < n * 36; it += 64) {
-        const int r = it / 36, i = it - 36 * r;
-        const int64_t src = s_src[r];
-        if (src < 0) continue;
-        const uint8_t *p = base + src;
-        const int t = s_st[r];
-        if (i >= 32) {
-            const int b = i - 32;
-            const uint8_t *sp = p + SCALE_OFF + (isv ? ((t >> 2) * 4 + b) * 8 + (t & 3) * 2 : (4 * t + b) * 2);
-            *reinterpret_cast<uint16_t *>(rows + r * PITCH + 128 + 2 * b) = *reinterpret_cast<const uint16_t *>(sp);
-        } else if (isv) {
-            const u32x4 c = *reinterpret_cast<const u32x4 *>(p + (i >> 4) * 1024 + (t >> 2) * 256 + (i & 15) * 16);
-            uint32_t v = 0;
+    const int n = s_n;
+    if (n == 0) return;
+    const int pairs = a.layers * a.Hkv;
+    if (s_ascending) {
+        for (int p = blockIdx.y * 4 + wv; p < pairs; p += gridDim.y * 4) {
+            const int layer = p / a.Hkv;
+            const int64_t head = (int64_t)(p - layer * a.Hkv) * a.chs;
+            uint8_t *const kb = (a.list ? a.k[layer] : a.k[0] + layer * a.layer_stride) + head;
+            uint8_t *const vb = (a.list ? a.v[layer] : a.v[0] + layer * a.layer_stride) + head;
+            for (int u = lane; u < 9 * n; u += 64) {
+                const int r = u / 9, c = u - 9 * r;
+                const int tok = s_tok[r];
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + s_src[r] + piece_off(c, tok & 15));
+                piece_store(kb + s_dst[r], c, tok & 15, tok >> 8, x);
+            }
+            for (int u = lane; u < CR_QUAD * s_nquad; u += 64) {
+                const int q = u / CR_QUAD, j = u - CR_QUAD * q;
+                const int64_t sub = s_quad[q] & ~(int64_t)15;
+                const int at = j < 32 ? (j >> 4) * 1024 + (j & 15) * 16 : SCALE_OFF + (j - 32) * 16;
+                const int per = j < 32 ? 256 : 32;  // bytes of a quad
+                u32x4 *const to = reinterpret_cast<u32x4 *>(vb + sub + at + per * (int)(s_quad[q] & 3));
+                u32x4 x = *to, y[4];
+                int t[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v |= ((c[e] >> (8 * (t & 3))) & 0xFFu) << (8 * e);
-            *reinterpret_cast<uint32_t *>(rows + r * PITCH + 4 * i) = v;
-        } else {
-            *reinterpret_cast<uint32_t *>(rows + r * PITCH + 4 * i) =
-                *reinterpret_cast<const uint32_t *>(p + (i >> 4) * 1024 + t * 64 + (i & 15) * 4);
-        }
-    }
-    __syncthreads();  // every load has completed
-    for (int it = lane; it < n * 36; it += 64) {
-        const int r = it / 36, i = it - 36 * r;
-        if (s_src[r] < 0) continue;
-        uint8_t *p = base + s_dst[r];
-        const int t = s_dt[r];
-        if (i >= 32) {
-            const int b = i - 32;
-            uint8_t *sp = p + SCALE_OFF + (isv ? ((t >> 2) * 4 + b) * 8 + (t & 3) * 2 : (4 * t + b) * 2);
-            *reinterpret_cast<uint16_t *>(sp) = *reinterpret_cast<const uint16_t *>(rows + r * PITCH + 128 + 2 * b);
-        } else {
-            const uint32_t v = *reinterpret_cast<const uint32_t *>(rows + r * PITCH + 4 * i);
-            if (isv) {
-                uint8_t *q = p + (i >> 4) * 1024 + (t >> 2) * 256 + (i & 15) * 16 + (t & 3);
+                for (int w = 0; w < 4; ++w) {  // (a token without a row takes its own bytes)
+                    const int r = s_row[q][w];
+                    t[w] = r < 0 ? w : s_tok[r] & 15;
+                    const uint8_t *from = r < 0 ? reinterpret_cast<const uint8_t *>(to)
+                                                : vb + s_src[r] + at + per * (t[w] >> 2);
+                    y[w] = *reinterpret_cast<const u32x4 *>(from);
+                }
+                if (j < 32) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) q[4 * e] = (uint8_t)(v >> (8 * e));
-            } else {
-                *reinterpret_cast<uint32_t *>(p + (i >> 4) * 1024 + t * 64 + (i & 15) * 4) = v;
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t v = 0;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) v |= ((y[w][e] >> (8 * (t[w] & 3))) & 0xFFu) << (8 * w);
+                        x[e] = v;
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t d = t[w] & 2 ? y[w][2 * b + 1] : y[w][2 * b];
+                            h[w] = t[w] & 1 ? d >> 16 : d & 0xFFFFu;
+                        }
+                        x[2 * b] = h[0] | h[1] << 16;
+                        x[2 * b + 1] = h[2] | h[3] << 16;
+                    }
+                }
+                *to = x;
             }
         }
+        return;
+    }
+    // any order: the workgroup takes one pair at a time, all rows through LDS
+    for (int p = blockIdx.y; p < pairs; p += gridDim.y) {
+        const int layer = p / a.Hkv;
+        const int64_t head = (int64_t)(p - layer * a.Hkv) * a.chs;
+        uint8_t *const kb = (a.list ? a.k[layer] : a.k[0] + layer * a.layer_stride) + head;
+        uint8_t *const vb = (a.list ? a.v[layer] : a.v[0] + layer * a.layer_stride) + head;
+        for (int u = threadIdx.x; u < n * CR_PIECES; u += 256) {
+            const int r = u / CR_PIECES, c = u - CR_PIECES * r;
+            rows[u] = *reinterpret_cast<const u32x4 *>((c < 9 ? kb : vb) + s_src[r] + piece_off(c, s_tok[r] & 15));
+        }
+        __syncthreads();
+        for (int u = threadIdx.x; u < n * CR_PIECES; u += 256) {
+            const int r = u / CR_PIECES, c = u - CR_PIECES * r;
+            piece_store((c < 9 ? kb : vb) + s_dst[r], c, s_tok[r] & 15, s_tok[r] >> 8, rows[u]);
+        }
+        __syncthreads();  // rows[] is filled again
     }
 }
 
@@ -182,15 +364,14 @@ extern "C" hipError_t gfx906_fa_amd_read_rows(
         return hipErrorInvalidValue;
     }
     const uint64_t os = (uint64_t)(k_out_row_stride | k_out_head_stride | v_out_row_stride | v_out_head_stride);
-    const uint64_t align = out_dtype == GFA_DTYPE_F32 ? 15u : 15u;
     if (!plane_ok(k_cache, v_cache, cache_block_stride, cache_head_stride) ||
-        (((uintptr_t)k_out | (uintptr_t)v_out) & align) || (os & 7u)) {
+        (((uintptr_t)k_out | (uintptr_t)v_out) & 15u) || (os & 7u)) {
         fprintf(stderr, "[gfx906_fa_amd] read_rows: cache and outputs must be 16-byte aligned, output strides multiples "
                         "of 8 elements\n");
         return hipErrorInvalidValue;
     }
     if (num_rows == 0) return hipSuccess;
-    const int64_t blocks = (num_rows * num_kv_heads + 3) / 4;
+    const int64_t blocks = ((num_rows + 15) / 16 * num_kv_heads + 3) / 4;
     if (blocks > 0x7FFFFFFF) {
         fprintf(stderr, "[gfx906_fa_amd] read_rows: too many rows\n");
         return hipErrorInvalidValue;
@@ -231,8 +412,8 @@ extern "C" hipError_t gfx906_fa_amd_compact_draft_rows(
         return hipErrorInvalidValue;
     }
     if (num_seqs == 0 || num_layers == 0 || accepted_cols == 0) return hipSuccess;
-    if ((int64_t)num_seqs * num_kv_heads > 0x7FFFFFFF || num_layers > 65535) {
-        fprintf(stderr, "[gfx906_fa_amd] compact_draft_rows: too many sequences or layers\n");
+    if ((int64_t)num_layers * num_kv_heads > (1 << 24)) {
+        fprintf(stderr, "[gfx906_fa_amd] compact_draft_rows: too many layers\n");
         return hipErrorInvalidValue;
     }
     CompactArgs a{};
@@ -252,14 +433,20 @@ extern "C" hipError_t gfx906_fa_amd_compact_draft_rows(
     a.Hkv = num_kv_heads;
     a.block_size = block_size;
     a.list = list ? 1 : 0;
-    const size_t lds = (size_t)accepted_cols * 144;
+    const size_t lds = (size_t)accepted_cols * CR_PIECES * 16;
+    static_assert(MAX_DRAFT * CR_PIECES * 16 + 3 * 512 <= 64 * 1024, "LDS of a workgroup");
     for (int l0 = 0; l0 < num_layers; l0 += list ? LAYERS : num_layers) {
         const int nl = list ? min(LAYERS, num_layers - l0) : num_layers;
         for (int i = 0; i < (list ? nl : 1); ++i) {
             a.k[i] = list ? k_layers[l0 + i] : k_cache;
             a.v[i] = list ? v_layers[l0 + i] : v_cache;
         }
-        compact_rows_kernel<<<dim3(num_seqs * num_kv_heads, 2, nl), 64, lds, stream>>>(a);
+        a.layers = nl;
+        // (layer, kv-head) pairs a wave takes: more where they alone fill the device
+        const int64_t pairs = (int64_t)nl * num_kv_heads;
+        const int64_t each = max((int64_t)1, min((int64_t)8, pairs * num_seqs / CR_WAVES));
+        const int64_t wgs = min((pairs + 4 * each - 1) / (4 * each), (int64_t)65535);
+        compact_rows_kernel<<<dim3(num_seqs, (unsigned)wgs), 256, lds, stream>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -40,7 +40,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -614,33 +613,43 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
 MAX_TREE_NODES = 64
 
 
-def _on(dev: torch.device):
-    """The device current for a call's launches (no-op where it is already)."""
-    return nullcontext() if dev.index is None or torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+_get_device = torch._C._cuda_getDevice
 
 
-def _all_on(dev: torch.device, tensors, names: str) -> None:
+def _all_on(i: int, tensors, names: str) -> None:
+    """Names the tensor that is not on device i."""
     for t, n in zip(tensors, names.split()):
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != i:
             _cuda(t, n)
-            raise RuntimeError(f"{n} must be on {dev}, got {t.device}")
+            raise RuntimeError(f"{n} must be on cuda:{i}, got {t.device}")
 
 
 def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, max_query_len, max_seq_len, scale,
             soft_cap, alibi_slopes, tree_mask, out, workspace, q_abs_offset, causal, out_dtype):
     """scored_paged_attention and tree_attention: checks and the one call."""
-    if not query.is_cuda:
+    at = query.get_device()
+    if at < 0:
         _cuda(query, "query")
-    dev = query.device
-    _all_on(dev, (key_cache, value_cache, block_table, seq_lens, query_start_loc, alibi_slopes, tree_mask, out,
-                  workspace, q_abs_offset),
-            "key_cache value_cache block_table seq_lens query_start_loc alibi_slopes tree_mask out workspace q_abs_offset")
-    if query.dtype not in (torch.float16, torch.bfloat16):
+    if not (key_cache.get_device() == value_cache.get_device() == block_table.get_device() == seq_lens.get_device()
+            == query_start_loc.get_device() == at) or any(
+                t is not None and t.get_device() != at for t in (alibi_slopes, tree_mask, out, workspace, q_abs_offset)):
+        _all_on(at, (key_cache, value_cache, block_table, seq_lens, query_start_loc, alibi_slopes, tree_mask, out,
+                     workspace, q_abs_offset),
+                "key_cache value_cache block_table seq_lens query_start_loc alibi_slopes tree_mask out workspace "
+                "q_abs_offset")
+    if _get_device() != at:  # the plan counts the current device's CUs, and the launches go there
+        with torch.cuda.device(at):
+            return _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, max_query_len,
+                           max_seq_len, scale, soft_cap, alibi_slopes, tree_mask, out, workspace, q_abs_offset, causal,
+                           out_dtype)
+    dev, dt = query.device, query.dtype
+    qdt = _DT.get(dt)
+    if not qdt:  # fp32's code is 0
         raise RuntimeError("query must be fp16 or bf16")
-    qdt = _DT[query.dtype]
-    if query.dim() != 3 or query.shape[2] != 128:
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != 128:
         raise RuntimeError("query must be [num_tokens, Hq, 128]")
-    T, Hq, D = query.shape
+    T, Hq, D = shape
     soft_cap = float(soft_cap)
     if not 0.0 <= soft_cap < float("inf"):
         raise RuntimeError(f"soft_cap must be 0 (none) or positive and finite, got {soft_cap}")
@@ -649,10 +658,10 @@ def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_lo
             raise RuntimeError("soft_cap and alibi_slopes exclude each other")
         if alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (Hq,) or not alibi_slopes.is_contiguous():
             raise RuntimeError("alibi_slopes must be contiguous fp32 [Hq]")
-    if out_dtype is not None and out_dtype not in (query.dtype, torch.float32):
+    if out_dtype is not None and out_dtype not in (dt, torch.float32):
         raise RuntimeError("out must be of the query dtype or fp32")
     if T == 0:  # no query rows (an empty tensor's strides are arbitrary)
-        return out if out is not None else torch.empty((0, Hq, D), dtype=out_dtype or query.dtype, device=dev)
+        return out if out is not None else torch.empty((0, Hq, D), dtype=out_dtype or dt, device=dev)
     qts, qhs, qs = query.stride()
     if qs != 1:
         raise RuntimeError("query rows must be contiguous")
@@ -669,7 +678,8 @@ def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_lo
     if block_table.shape[0] < B or query_start_loc.shape[0] < B + 1:
         raise RuntimeError("block_table / query_start_loc shorter than seq_lens")
     if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 1 or tree_mask.shape[0] < T or not tree_mask.is_contiguous():
+        if (tree_mask.dtype != torch.int64 or tree_mask.dim() != 1 or tree_mask.shape[0] < T
+                or not tree_mask.is_contiguous()):
             raise RuntimeError("tree_mask must be contiguous int64 [num_tokens]")
         if max_query_len > MAX_TREE_NODES:
             raise RuntimeError(f"a tree has at most {MAX_TREE_NODES} nodes (max_query_len {max_query_len})")
@@ -677,29 +687,33 @@ def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_lo
         _check(q_abs_offset.dtype == torch.int32 and q_abs_offset.is_contiguous()
                and q_abs_offset.shape[0] >= B, "q_abs_offset must be int32 [B]")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=out_dtype or query.dtype, device=dev)
-    oshape, ostrides = out.shape, out.stride()
-    if out.dtype not in (query.dtype, torch.float32):
-        raise RuntimeError("out must be of the query dtype or fp32")
-    if len(oshape) != 3 or oshape[1] != Hq or oshape[2] != D or oshape[0] < T or ostrides[2] != 1:
-        raise RuntimeError("out must be [num_tokens, Hq, 128]")
+        out = torch.empty((T, Hq, D), dtype=out_dtype or dt, device=dev)
+        odt, ots, ohs = _DT[out_dtype or dt], Hq * D, D
+    else:
+        oshape, (ots, ohs, os) = out.shape, out.stride() if out.dim() == 3 else (0, 0, 0)
+        if out.dtype not in (dt, torch.float32):
+            raise RuntimeError("out must be of the query dtype or fp32")
+        if len(oshape) != 3 or oshape[1] != Hq or oshape[2] != D or oshape[0] < T or os != 1:
+            raise RuntimeError("out must be [num_tokens, Hq, 128]")
+        odt = _DT[out.dtype]
     if B == 0:
         return out
-    L = _load()
-    with _on(dev):
-        need = L.gfx906_fa_amd_paged_attention_workspace_size(B, T, Hq, Hkv, D, max_query_len, max_seq_len)
-        if workspace is None or (workspace.nbytes < need and workspace.nbytes < plan_info(
-                B, T, Hq, Hkv, max_query_len, max_seq_len, D)["img_offset"]):
-            workspace = new_workspace(need, dev)
-        ws_ptr = workspace.data_ptr()
-        if ws_ptr % 256 or not workspace.is_contiguous():
-            raise RuntimeError("workspace must be contiguous and 256-byte aligned")
-        err = L.gfx906_fa_amd_scored_paged_attention(
-            query.data_ptr(), qdt, qts, qhs, key_cache.data_ptr(), value_cache.data_ptr(), cbs, chs,
-            block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), query_start_loc.data_ptr(),
-            _ptr(q_abs_offset), 1 if causal else 0, soft_cap, _ptr(alibi_slopes), _ptr(tree_mask), B, T, Hq, Hkv, D, bs,
-            int(max_query_len), int(max_seq_len), float(scale), out.data_ptr(), _DT[out.dtype], ostrides[0], ostrides[1],
-            ws_ptr, workspace.nbytes, _stream(dev))
+    L = _lib
+    need = L.gfx906_fa_amd_paged_attention_workspace_size(B, T, Hq, Hkv, D, max_query_len, max_seq_len)
+    have = 0 if workspace is None else workspace.nbytes
+    if have < need and (have == 0 or have < plan_info(B, T, Hq, Hkv, max_query_len, max_seq_len, D)["img_offset"]):
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        have = need
+    ws_ptr = workspace.data_ptr()
+    if ws_ptr % 256 or not workspace.is_contiguous():
+        raise RuntimeError("workspace must be contiguous and 256-byte aligned")
+    err = L.gfx906_fa_amd_scored_paged_attention(
+        query.data_ptr(), qdt, qts, qhs, key_cache.data_ptr(), value_cache.data_ptr(), cbs, chs,
+        block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), query_start_loc.data_ptr(),
+        None if q_abs_offset is None else q_abs_offset.data_ptr(), 1 if causal else 0, soft_cap,
+        None if alibi_slopes is None else alibi_slopes.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(),
+        B, T, Hq, Hkv, D, bs, int(max_query_len), int(max_seq_len), float(scale), out.data_ptr(), odt, ots, ohs, ws_ptr, have,
+        _stream(dev))
     if err:
         _ok(err, "gfx906_fa_amd_scored_paged_attention")
     return out
@@ -774,49 +788,67 @@ def qk_norm_rope_and_cache_q8_kv(positions: torch.Tensor, query: torch.Tensor, k
     fp32 and rounded once; the stored key and the value go to the cache as Q8_0
     at slot_mapping (< 0 skips).  One launch.  Rows at positions outside
     [0, max_position) are normed and not rotated."""
-    if not query.is_cuda:
+    at = query.get_device()
+    if at < 0:
         _cuda(query, "query")
-    dev = query.device
-    _all_on(dev, (positions, key, value, query_weight, key_weight, cos_sin_cache, slot_mapping, key_cache, value_cache),
-            "positions key value query_weight key_weight cos_sin_cache slot_mapping key_cache value_cache")
+    if not (positions.get_device() == key.get_device() == value.get_device() == query_weight.get_device()
+            == key_weight.get_device() == cos_sin_cache.get_device() == slot_mapping.get_device()
+            == key_cache.get_device() == value_cache.get_device() == at):
+        _all_on(at, (positions, key, value, query_weight, key_weight, cos_sin_cache, slot_mapping, key_cache, value_cache),
+                "positions key value query_weight key_weight cos_sin_cache slot_mapping key_cache value_cache")
+    if _get_device() != at:
+        with torch.cuda.device(at):
+            return qk_norm_rope_and_cache_q8_kv(positions, query, key, value, query_weight, key_weight, eps, cos_sin_cache,
+                                                is_neox, slot_mapping, key_cache, value_cache, rot_dim)
     dt = query.dtype
-    _check(dt in (torch.float16, torch.bfloat16) and key.dtype == dt and value.dtype == dt,
-           "query/key/value must share dtype fp16 or bf16")
-    _check(query.dim() == 3 and key.dim() == 3 and value.shape == key.shape and query.shape[0] == key.shape[0],
-           "query must be [T, Hq, D], key/value [T, Hkv, D]")
-    _check(positions.dtype == torch.int64 and positions.dim() == 1 and positions.shape[0] == query.shape[0],
-           "positions must be int64 [num_tokens]")
-    _check(slot_mapping.dtype == torch.int64 and slot_mapping.dim() == 1 and slot_mapping.shape[0] == query.shape[0],
-           "slot_mapping must be int64 [num_tokens]")
-    _check(cos_sin_cache.dtype in _DT and cos_sin_cache.dim() == 2 and cos_sin_cache.stride(1) == 1,
-           "cos_sin_cache must be [max_position, rot_dim] with contiguous rows")
-    T, Hq, D = query.shape
-    Hkv = key.shape[1]
-    _check(D == 128 and key.shape[2] == 128, "head_size must be 128")
-    for w, n in ((query_weight, "query_weight"), (key_weight, "key_weight")):
-        _check(w.dtype == dt and tuple(w.shape) == (128,) and w.is_contiguous(), f"{n} must be [128] of the query dtype")
-    _check(float(eps) >= 0.0, "eps must be >= 0")
+    qdt, cdt = _DT.get(dt), _DT.get(cos_sin_cache.dtype)
+    if not qdt or key.dtype != dt or value.dtype != dt:  # fp32's code is 0
+        raise RuntimeError("query/key/value must share dtype fp16 or bf16")
+    qshape, kshape = query.shape, key.shape
+    if len(qshape) != 3 or len(kshape) != 3 or value.shape != kshape or qshape[0] != kshape[0]:
+        raise RuntimeError("query must be [T, Hq, D], key/value [T, Hkv, D]")
+    T, Hq, D = qshape
+    Hkv = kshape[1]
+    if D != 128 or kshape[2] != 128:
+        raise RuntimeError("head_size must be 128")
+    if positions.dtype != torch.int64 or positions.shape != (T,):
+        raise RuntimeError("positions must be int64 [num_tokens]")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,):
+        raise RuntimeError("slot_mapping must be int64 [num_tokens]")
+    if cdt is None or cos_sin_cache.dim() != 2 or cos_sin_cache.stride(1) != 1:
+        raise RuntimeError("cos_sin_cache must be [max_position, rot_dim] with contiguous rows")
+    if query_weight.dtype != dt or query_weight.shape != (128,) or not query_weight.is_contiguous():
+        raise RuntimeError("query_weight must be [128] of the query dtype")
+    if key_weight.dtype != dt or key_weight.shape != (128,) or not key_weight.is_contiguous():
+        raise RuntimeError("key_weight must be [128] of the query dtype")
+    if not eps >= 0.0:
+        raise RuntimeError("eps must be >= 0")
     if T == 0:  # nothing to do (an empty tensor's strides are arbitrary)
         return
-    if query.stride(2) != 1 or key.stride(2) != 1 or value.stride(2) != 1:
+    (qts, qhs, qs), (kts, khs, ks), (vts, vhs, vs) = query.stride(), key.stride(), value.stride()
+    if qs != 1 or ks != 1 or vs != 1:
         raise RuntimeError("query, key and value rows must be contiguous")
-    rot = cos_sin_cache.shape[1] if rot_dim is None else int(rot_dim)
-    _check(rot <= cos_sin_cache.shape[1], f"rot_dim={rot} exceeds the {cos_sin_cache.shape[1]} columns of cos_sin_cache")
+    npos, rot = cos_sin_cache.shape
+    if rot_dim is not None:
+        if rot_dim > rot:
+            raise RuntimeError(f"rot_dim={rot_dim} exceeds the {rot} columns of cos_sin_cache")
+        rot = int(rot_dim)
     bs, Hc, cbs, chs = _plane_info(key_cache, value_cache)
-    if Hc != Hkv:
+    if Hc != Hkv or Hkv == 0:
         raise RuntimeError(f"cache Hkv mismatch: got {Hc} vs key Hkv={Hkv}")
     if Hq % Hkv:
         raise RuntimeError(f"heads_q={Hq} must be divisible by heads_kv={Hkv}")
-    pos = positions.contiguous()
-    sm = slot_mapping.contiguous()
-    with _on(dev):
-        err = _load().gfx906_fa_amd_qk_norm_rope_cache_write_kv(
-            _ptr(query), _ptr(key), _ptr(value), _ptr(query_weight), _ptr(key_weight), float(eps), _DT[dt], _ptr(pos),
-            _ptr(cos_sin_cache), _DT[cos_sin_cache.dtype], cos_sin_cache.stride(0), cos_sin_cache.shape[0], rot,
-            1 if is_neox else 0, _ptr(sm), _ptr(key_cache), _ptr(value_cache), T, Hq, Hkv, D, bs,
-            query.stride(0), query.stride(1), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
-            cbs, chs, _stream(dev))
-    _ok(err, "gfx906_fa_amd_qk_norm_rope_cache_write_kv")
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.contiguous()
+    err = _lib.gfx906_fa_amd_qk_norm_rope_cache_write_kv(
+        query.data_ptr(), key.data_ptr(), value.data_ptr(), query_weight.data_ptr(), key_weight.data_ptr(), float(eps), qdt,
+        positions.data_ptr(), cos_sin_cache.data_ptr(), cdt, cos_sin_cache.stride(0), npos, rot, 1 if is_neox else 0,
+        slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), T, Hq, Hkv, D, bs, qts, qhs, kts, khs, vts,
+        vhs, cbs, chs, _stream(query.device))
+    if err:
+        _ok(err, "gfx906_fa_amd_qk_norm_rope_cache_write_kv")
 
 
 def read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -827,10 +859,15 @@ def read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_
     fp32), int8 * scale rounded once.  Slots outside the cache (< 0 too) give
     zeros.  ``k_out`` / ``v_out`` are filled where given (that shape and dtype,
     contiguous last dim, rows 16-byte aligned)."""
-    if not slot_mapping.is_cuda:
+    at = slot_mapping.get_device()
+    if at < 0:
         _cuda(slot_mapping, "slot_mapping")
-    dev = slot_mapping.device
-    _all_on(dev, (key_cache, value_cache, k_out, v_out), "key_cache value_cache k_out v_out")
+    if not (key_cache.get_device() == value_cache.get_device() == at) or any(
+            t is not None and t.get_device() != at for t in (k_out, v_out)):
+        _all_on(at, (key_cache, value_cache, k_out, v_out), "key_cache value_cache k_out v_out")
+    if _get_device() != at:
+        with torch.cuda.device(at):
+            return read_cache_q8_kv(slot_mapping, key_cache, value_cache, dtype, k_out, v_out)
     if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1:
         raise RuntimeError("slot_mapping must be int64 [num_tokens]")
     odt = _DT.get(dtype)
@@ -838,21 +875,31 @@ def read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_
         raise RuntimeError("dtype must be fp16, bf16 or fp32")
     bs, Hkv, cbs, chs = _plane_info(key_cache, value_cache)
     T = slot_mapping.shape[0]
-    outs = []
-    for o, n in ((k_out, "k_out"), (v_out, "v_out")):
-        if o is None:
-            o = torch.empty((T, Hkv, 128), dtype=dtype, device=dev)
-        elif o.shape != (T, Hkv, 128) or o.dtype != dtype or (T and o.stride(2) != 1):
-            raise RuntimeError(f"{n} must be [num_tokens, Hkv, 128] of dtype {dtype} with contiguous rows")
-        outs.append(o)
-    k, v = outs
+    dev = slot_mapping.device
+    if k_out is None and v_out is None:
+        # one allocation for both
+        kv = torch.empty((2, T, Hkv, 128), dtype=dtype, device=dev)
+        k, v = kv.unbind(0)
+        kts = vts = Hkv * 128
+        khs = vhs = 128
+    else:
+        k, v = k_out, v_out
+        strides = []
+        for o, n in ((k, "k_out"), (v, "v_out")):
+            if o is None:
+                o = torch.empty((T, Hkv, 128), dtype=dtype, device=dev)
+                k, v = (o, v) if n == "k_out" else (k, o)
+            elif o.shape != (T, Hkv, 128) or o.dtype != dtype or (T and o.stride(2) != 1):
+                raise RuntimeError(f"{n} must be [num_tokens, Hkv, 128] of dtype {dtype} with contiguous rows")
+            strides += o.stride()[:2]
+        kts, khs, vts, vhs = strides
     if T == 0 or Hkv == 0:
         return k, v
-    sm = slot_mapping.contiguous()
-    with _on(dev):
-        err = _load().gfx906_fa_amd_read_rows(
-            key_cache.data_ptr(), value_cache.data_ptr(), sm.data_ptr(), k.data_ptr(), v.data_ptr(), odt, T, Hkv, 128, bs,
-            key_cache.shape[0], cbs, chs, k.stride(0), k.stride(1), v.stride(0), v.stride(1), _stream(dev))
+    if not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.contiguous()
+    err = _lib.gfx906_fa_amd_read_rows(
+        key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(), k.data_ptr(), v.data_ptr(), odt, T, Hkv,
+        128, bs, key_cache.shape[0], cbs, chs, kts, khs, vts, vhs, _stream(dev))
     if err:
         _ok(err, "gfx906_fa_amd_read_rows")
     return k, v
@@ -873,52 +920,62 @@ def compact_draft_rows(kv_caches, block_table: torch.Tensor, seq_lens: torch.Ten
     ``kv_caches``: one stacked tensor, uint8 [layers, NB, 2, Hkv, bs/16*2176],
     or a sequence of (key_cache, value_cache) planes, one pair per layer, of
     one shape and one set of strides.  Sequences must not share draft pages."""
-    list_ptrs = (None, None)
+    kp = vp = None
     if isinstance(kv_caches, torch.Tensor):
-        if kv_caches.dim() != 5 or kv_caches.shape[2] != 2 or kv_caches.dtype != torch.uint8:
+        shape = kv_caches.shape
+        if len(shape) != 5 or shape[2] != 2 or kv_caches.dtype != torch.uint8:
             raise RuntimeError("kv_caches must be uint8 [layers, num_blocks, 2, Hkv, block_size/16*2176]")
-        layers, lstride = kv_caches.shape[0], kv_caches.stride(0)
+        layers, nb, _, Hkv, page = shape
+        lstride, cbs, plane, chs, last = kv_caches.stride()
+        subs, rest = divmod(page, SUBPAGE_BYTES)
+        if rest or last != 1:
+            raise RuntimeError("pages must be contiguous, a multiple of 2176 bytes")
+        bs, at = subs * SUBPAGE_TOKENS, kv_caches.get_device()
         if layers == 0:
             return
-        kc, vc = kv_caches[0, :, 0], kv_caches[0, :, 1]
+        k0 = kv_caches.data_ptr()
+        v0 = k0 + plane
     else:
-        pairs = list(kv_caches)
-        layers, lstride = len(pairs), 0
+        pairs = kv_caches = list(kv_caches)
+        layers, lstride, k0, v0 = len(pairs), 0, None, None
         if layers == 0:
             return
-        kc, vc = pairs[0]
-        shape, strides, dev0 = kc.shape, kc.stride(), kc.device
+        kc = pairs[0][0]
+        bs, Hkv, cbs, chs = _plane_info(*pairs[0])
+        shape, strides, at, nb = kc.shape, kc.stride(), kc.get_device(), kc.shape[0]
         for k, v in pairs:
-            for t in (k, v):
-                if t.shape != shape or t.stride() != strides or t.dtype != torch.uint8 or t.device != dev0:
-                    raise RuntimeError("every layer's planes must be uint8 of one shape, set of strides and device")
-        list_ptrs = tuple((ctypes.c_void_p * layers)(*(p[i].data_ptr() for p in pairs)) for i in range(2))
-    bs, Hkv, cbs, chs = _plane_info(kc, vc)
-    if not kc.is_cuda:
-        _cuda(kc, "kv_caches")
-    dev = kc.device
-    _all_on(dev, (block_table, seq_lens, query_start_loc, accepted, num_accepted),
-            "block_table seq_lens query_start_loc accepted num_accepted")
+            if not (k.shape == v.shape == shape and k.stride() == v.stride() == strides
+                    and k.dtype == v.dtype == torch.uint8 and k.get_device() == v.get_device() == at):
+                raise RuntimeError("every layer's planes must be uint8 of one shape, set of strides and device")
+        kp, vp = ((ctypes.c_void_p * layers)(*[p[i].data_ptr() for p in pairs]) for i in range(2))
+    if at < 0:
+        raise RuntimeError("kv_caches must be CUDA/HIP")
+    if not (block_table.get_device() == seq_lens.get_device() == query_start_loc.get_device() == accepted.get_device()
+            == num_accepted.get_device() == at):
+        _all_on(at, (block_table, seq_lens, query_start_loc, accepted, num_accepted),
+                "block_table seq_lens query_start_loc accepted num_accepted")
+    if _get_device() != at:
+        with torch.cuda.device(at):
+            return compact_draft_rows(kv_caches, block_table, seq_lens, query_start_loc, accepted, num_accepted)
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
         raise RuntimeError("block_table must be int32 [num_seqs, max_blocks] with contiguous rows")
-    for t, n in ((seq_lens, "seq_lens"), (query_start_loc, "query_start_loc"), (num_accepted, "num_accepted")):
+    for t in (seq_lens, query_start_loc, num_accepted):
         if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-            raise RuntimeError(f"{n} must be contiguous int32")
+            raise RuntimeError("seq_lens, query_start_loc and num_accepted must be contiguous int32")
     B = seq_lens.shape[0]
     if block_table.shape[0] < B or query_start_loc.shape[0] < B + 1 or num_accepted.shape[0] < B:
         raise RuntimeError("block_table / query_start_loc / num_accepted shorter than seq_lens")
     if accepted.dtype != torch.int32 or accepted.dim() != 2 or accepted.shape[0] < B or accepted.stride(1) != 1:
         raise RuntimeError("accepted must be int32 [num_seqs, at most 64] with contiguous rows")
-    if accepted.shape[1] > MAX_TREE_NODES:
-        raise RuntimeError(f"accepted has at most {MAX_TREE_NODES} columns, got {accepted.shape[1]}")
-    if B == 0 or accepted.shape[1] == 0 or Hkv == 0:
+    cols = accepted.shape[1]
+    if cols > MAX_TREE_NODES:
+        raise RuntimeError(f"accepted has at most {MAX_TREE_NODES} columns, got {cols}")
+    if B == 0 or cols == 0 or Hkv == 0 or bs == 0:
         return
-    with _on(dev):
-        err = _load().gfx906_fa_amd_compact_draft_rows(
-            list_ptrs[0], list_ptrs[1], kc.data_ptr(), vc.data_ptr(), lstride, layers, cbs, chs, kc.shape[0],
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
-            query_start_loc.data_ptr(), accepted.data_ptr(), accepted.stride(0), accepted.shape[1],
-            num_accepted.data_ptr(), B, Hkv, 128, bs, _stream(dev))
+    err = _lib.gfx906_fa_amd_compact_draft_rows(
+        kp, vp, k0, v0, lstride, layers, cbs, chs, nb, block_table.data_ptr(), block_table.stride(0),
+        block_table.shape[1], seq_lens.data_ptr(), query_start_loc.data_ptr(), accepted.data_ptr(), accepted.stride(0),
+        cols, num_accepted.data_ptr(), B, Hkv, 128, bs, _stream(accepted.device))
     if err:
         _ok(err, "gfx906_fa_amd_compact_draft_rows")
 

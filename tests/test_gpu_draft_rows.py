@@ -249,3 +249,25 @@ def test_tree_step_from_projection_to_next_token(cap):
                                           soft_cap=cap)
     check(o2, *scored_oracle(new, cap=cap, out_eps=eps_of(torch.bfloat16)))
     assert np.isfinite(to_np_f32(o2)).all()
+
+
+@pytest.mark.parametrize("n,keep", [(64, 63), (64, 40), (30, 12), (25, 11)])
+def test_compact_long_paths(n, keep):
+    """Ascending paths of more rows than a wave holds at once, several of them
+    a target that a later row's source is next to."""
+    need_gpu()
+    announce(f"compact long {n} {keep}")
+    rng = np.random.default_rng(n + keep)
+    ctx, nq = [7, 33, 64], [n] * 3
+    bt, nb = _tables(rng, [c + n for c in ctx], 16)
+    acc = np.full((3, 64), -1, np.int32)
+    for s in range(3):
+        acc[s, :keep] = np.sort(rng.permutation(n)[:keep]) if s else np.arange(n - keep, n)
+    stack = torch.randint(0, 256, (2, nb, 2, 3, 2176), dtype=torch.uint8, device=DEV)
+    want = stack.cpu().numpy().copy()
+    for layer in want:
+        _compact_ref(layer, bt, ctx, nq, acc, [keep] * 3)
+    t = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)  # noqa: E731
+    gfx906_fa.compact_draft_rows(stack, t(bt), t([c + n for c in ctx]), t(np.arange(4) * n), t(acc), t([keep] * 3))
+    torch.cuda.synchronize()
+    assert np.array_equal(stack.cpu().numpy(), want)

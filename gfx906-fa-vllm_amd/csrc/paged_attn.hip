@@ -1248,7 +1248,8 @@ __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void at
     // per wave: its merge rows (32 at most: 48-row tiles merge in two
     // passes), or (verify tiles) its LDS ring while it streams; rows past R
     // only lengthen the slice for the ring
-    constexpr int RA = NRG >= 2 ? cmax(R < 32 ? R : 32, (DEC_RING * DEC_RING_SLOT + 4 * 132 - 1) / (4 * 132)) : R;
+    constexpr bool RING = NRG >= 2 || SC != SC_NONE;
+    constexpr int RA = RING ? cmax(R < 32 ? R : 32, (DEC_RING * DEC_RING_SLOT + 4 * 132 - 1) / (4 * 132)) : R;
     __shared__ float sm_o[NW][RA][128 + 4];
     __shared__ float sm_m[NW][R], sm_l[NW][R];
     int64_t u = u0;
@@ -1278,7 +1279,11 @@ __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void at
         if constexpr (SC != SC_NONE) load_score_rows<NRG, SC>(p, h, si.q0, si.nq, rc, si.sl, si.qa, i16, sr, lim);
         WaveAcc<NRG> acc;
         acc_init(acc);
-        if constexpr (NRG >= 2) {  // verify tiles: sub-pages staged through this wave's sm_o slice
+        // verify tiles and the scored forms: sub-pages staged through this
+        // wave's sm_o slice.  (One row group of the scored forms with two
+        // sub-pages in registers instead, 64 of them: 20 spilled, 32 x 2K-16K
+        // capped 100 us.)
+        if constexpr (RING) {
             static_assert(sizeof(sm_o[0]) >= DEC_RING * DEC_RING_SLOT, "ring fits the wave's slice");
             stream_range_lds<NRG, DEC_RING, SC>(acc, p, s, h, 16 * a, min(16 * b, si.kv_lim), qf, lim, sr, lane, i16,
                                                 g, j0, jstep, reinterpret_cast<uint8_t *>(&sm_o[wv][0][0]));
@@ -1725,6 +1730,9 @@ __device__ __forceinline__ void pf_dequant_v(const PfRaw &r, uint8_t *vst, int s
 // them there), whose V rows are the caller's own.  An instance of its own: the
 // clearing of unseen V in the paged instance's copy loop cost the 32K prompt
 // 1 % (11.07 -> 11.2 ms), though it never ran there.
+#ifndef GFA_PF_QLDS
+#define GFA_PF_QLDS 4
+#endif
 template <int QDT, int ODT, bool VF16, bool MASK, int KS = 1, bool FLAT = false, int SC = SC_NONE>
 __global__ __launch_bounds__(64 * PF_WAVES)
 __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p) {
@@ -1735,7 +1743,12 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
     // (KS = 2 has room for the consumers' Q rows of its own; KS = 1 puts them
     // into the stages 1 and 2, free until the first tile has been written)
     constexpr int STAGES = NSTAGE * (PF_KBYTES + PF_VBYTES);
-    __shared__ __attribute__((aligned(16))) uint8_t lds[STAGES + (KS == 2 ? PF_CWAVES * PF_QBYTES : 0)];
+    // Q fragments that stay in LDS between the tiles (KS = 1: a lane's own 16
+    // bytes each; KS = 2: where the Q rows are).  The capped scores' temporaries do not fit beside all eight in
+    // registers: the compiler spilled two of them, and the QK waited for them
+    // to come back from memory in every tile.
+    constexpr int QLDS = SC == SC_CAP ? GFA_PF_QLDS : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[STAGES + PF_CWAVES * (KS == 2 ? PF_QBYTES : QLDS * 1024)];
     uint8_t *const ldsk = lds;
     uint8_t *const ldsv = lds + NSTAGE * PF_KBYTES;
     const int Hkv = p.Hkv;
@@ -2086,7 +2099,11 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
     // start, 48/8 heads, 42-token chunks: 4.7 -> 4.0 us with one workgroup
     // per kv-head, 6.0 -> 5.4 us with the device full (then the first reads
     // of all workgroups together, 26 MB, set the time).
-    half8_t qf[8];
+    half8_t qf[8 - QLDS];
+    constexpr int QSTEP = KS == 2 ? 32 : 1024;  // bytes between a lane's fragments in LDS
+    [[maybe_unused]] uint8_t *const qlds =
+        KS == 2 ? lds + STAGES + w * PF_QBYTES + (lane & 31) * PF_KPITCH + 32 * (8 - QLDS) + 16 * hb
+                : lds + STAGES + w * QLDS * 1024 + 16 * lane;
     {
         const float c = p.pf_qmul;  // a power of two: exact for fp16 / bf16 Q
         const int64_t qrow = (int64_t)(q0 + j) * p.q_ts + (int64_t)hq * p.q_hs;  // (rows past nrows: row j = 0)
@@ -2110,21 +2127,19 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-            qf[kk] = *reinterpret_cast<const half8_t *>(ql + (lane & 31) * PF_KPITCH + 32 * kk + 16 * hb);
-            if (!rvalid) qf[kk] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            half8_t f = *reinterpret_cast<const half8_t *>(ql + (lane & 31) * PF_KPITCH + 32 * kk + 16 * hb);
+            if (!rvalid) f = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            if (kk < 8 - QLDS) qf[kk < 8 - QLDS ? kk : 0] = f;
+            else *reinterpret_cast<half8_t *>(qlds + (kk - (8 - QLDS)) * QSTEP) = f;  // (the wave's own: in order)
         }
     }
-    // the scored forms' row: see ScoreRows
-    [[maybe_unused]] uint64_t tree = 0;
+    // the scored forms' row: see ScoreRows (its tree mask is loaded where a
+    // tile needs it: two registers less in every other)
     [[maybe_unused]] const int node0 = sl - nq;
     [[maybe_unused]] float slope = 0.0f;
-    if constexpr (SC == SC_BIAS) {
-        slope = rvalid ? p.slopes[hq] * LOG2E : 0.0f;
-    } else if constexpr (SC != SC_NONE) {
-        if (p.tree && rvalid) {
-            tree = tree_row(p, q0, j);
-            lim = min(lim, node0 - 1);
-        }
+    if constexpr (SC == SC_BIAS) slope = rvalid ? p.slopes[hq] * LOG2E : 0.0f;
+    if constexpr (SC == SC_TREE || SC == SC_CAP) {
+        if (p.tree && rvalid) lim = min(lim, node0 - 1);
     }
     int lim_min;  // smallest bound over the wave's rows: tiles below it need no mask
     {
@@ -2174,9 +2189,12 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
             }
             msp = __builtin_bit_cast(float16v_t, sp);
         }
+        half8_t ql[QLDS ? QLDS : 1];
+#pragma unroll
+        for (int kk = 0; kk < QLDS; ++kk) ql[kk] = *reinterpret_cast<const half8_t *>(qlds + kk * QSTEP);
 #pragma unroll
         for (int st = 0; st < PF_NST; ++st) {
-            if constexpr (SC == SC_CAP) {  // m is not linear in the capped score: it is subtracted in sv
+            if constexpr (SC == SC_CAP) {  // m is subtracted from the capped score
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sacc[st][e] = 0.0f;
             } else if constexpr (SC == SC_BIAS) {
@@ -2190,7 +2208,8 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
                 const half8_t a = *reinterpret_cast<const half8_t *>(kst + kread + 32 * st * PF_KPITCH + 32 * kk);
-                sacc[st] = mfma32(a, qf[kk], sacc[st]);
+                sacc[st] = mfma32(a, kk < 8 - QLDS ? qf[kk < 8 - QLDS ? kk : 0] : ql[kk < 8 - QLDS ? 0 : kk - (8 - QLDS)],
+                                  sacc[st]);
             }
         }
         // Schedule of this block: the K^ operand reads run two ahead of the
@@ -2198,13 +2217,22 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
         // the two in flight.  The compiler's own order waited for each pair
         // before its two MFMAs.  One box: cfg3 11.48 -> 11.20 ms, cfg4 5.93
         // -> 5.83 ms; three ahead: cfg3 11.22 ms, cfg4 5.90 ms.
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // DS reads
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 + QLDS, 0);  // DS reads
 #pragma unroll
         for (int i = 0; i < 8 * PF_NST - 1; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // DS read
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (SC == SC_CAP) {
+            // The cap (the QK gave 2 log2 e * scale / cap * q.k) and - m, in
+            // this half-step: its transcendental instructions (two of 8 cycles a
+            // score) run beside the other group's PV MFMAs.
+#pragma unroll
+            for (int st = 0; st < PF_NST; ++st)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sacc[st][e] = capped(sacc[st][e], p.cap_log2e, m_use);
+        }
     };
     // softmax and O += P V^ over tile kt (stage vst)
     auto sv = [&](int kt, const uint8_t *vst) __attribute__((always_inline)) {
@@ -2236,13 +2264,11 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
                     }
             }
         }
-        if constexpr (SC == SC_CAP) {  // (a product of 2 log2 e * scale / cap came out of the QK)
-#pragma unroll
-            for (int st = 0; st < PF_NST; ++st)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sacc[st][e] = capped(sacc[st][e], p.cap_log2e, m_use);
-        }
         if (kbase_t + PF_TK - 1 > lim_min) {  // uniform: tile crosses some row's bound
+            [[maybe_unused]] uint64_t tree = 0;
+            if constexpr (SC == SC_TREE || SC == SC_CAP) {
+                if (p.tree && rvalid) tree = tree_row(p, q0, j);
+            }
 #pragma unroll
             for (int st = 0; st < PF_NST; ++st)
 #pragma unroll

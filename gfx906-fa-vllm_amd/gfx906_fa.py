@@ -877,9 +877,8 @@ def read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_
     T = slot_mapping.shape[0]
     dev = slot_mapping.device
     if k_out is None and v_out is None:
-        # one allocation for both
-        kv = torch.empty((2, T, Hkv, 128), dtype=dtype, device=dev)
-        k, v = kv.unbind(0)
+        k = torch.empty((T, Hkv, 128), dtype=dtype, device=dev)
+        v = torch.empty((T, Hkv, 128), dtype=dtype, device=dev)
         kts = vts = Hkv * 128
         khs = vhs = 128
     else:

@@ -19,6 +19,11 @@ What differs, by design:
   * fp16 and bf16 models; head size 128 (the only size the reference's
     launchers accept, ``extension/gfx906_fa_launcher.cu:76-79``); any block
     size that is a multiple of 16.
+  * ``Gfx906FAScoredBackend`` (registered instead with GFX906_FA_SCORES=1)
+    takes the two score forms the reference refuses, a logits soft cap and ALiBi
+    slopes.  Both backends verify trees of drafts (``Gfx906FAMetadata.tree_mask``),
+    keep an accepted path (``keep_accepted_drafts``) and fuse q/k norms into the
+    rotation and cache write (``do_qk_norm_rope_and_kv_cache_update``).
 """
 from __future__ import annotations
 
@@ -68,6 +73,9 @@ class Gfx906FAMetadata:
     slot_mapping: torch.Tensor         # [num_tokens] int64
     use_cascade: bool = False
     common_prefix_len: int = 0
+    # int64 [num_tokens]: the step verifies a tree of drafts per sequence
+    # (gfx906_fa.tree_masks); None: causal rows
+    tree_mask: torch.Tensor | None = None
 
 
 def workspace_upper_bound(max_num_seqs: int, max_num_tokens: int, heads, max_seq_len: int = -1,
@@ -249,6 +257,18 @@ class Gfx906FABackend(AttentionBackend):
     def get_builder_cls() -> type["Gfx906FAMetadataBuilder"]:
         return Gfx906FAMetadataBuilder
 
+    @staticmethod
+    def keep_accepted_drafts(kv_caches, num_kv_heads: int, head_size: int, metadata: "Gfx906FAMetadata",
+                             accepted: torch.Tensor, num_accepted: torch.Tensor) -> None:
+        """After a tree step (``metadata``): the rows of the accepted drafts
+        (int32 [B, A] indices, int32 [B] counts, a path's root first) move
+        behind their context in every layer's cache (``kv_caches``: a list of the
+        layers' tensors, any layout ``q8_planes`` takes).  The next step's
+        seq_lens are ctx + num_accepted."""
+        gfx906_fa.compact_draft_rows([q8_planes(kv, num_kv_heads, head_size) for kv in kv_caches],
+                                     metadata.block_table, metadata.seq_lens, metadata.query_start_loc, accepted,
+                                     num_accepted)
+
     @classmethod
     def supports_head_size(cls, head_size: int) -> bool:
         return head_size == 128
@@ -361,6 +381,29 @@ class Gfx906FAImpl(AttentionImpl):
         sm = layer_slot_mapping if layer_slot_mapping.dtype == torch.int64 else layer_slot_mapping.to(torch.int64)
         gfx906_fa.rope_and_cache_q8_kv(pos, q, k, v, cos_sin_cache, is_neox, sm, kp, vp)
 
+    def do_qk_norm_rope_and_kv_cache_update(self, layer: AttentionLayer, query: torch.Tensor, key: torch.Tensor,
+                                            value: torch.Tensor, positions: torch.Tensor, query_weight: torch.Tensor,
+                                            key_weight: torch.Tensor, eps: float, cos_sin_cache: torch.Tensor,
+                                            is_neox: bool, kv_cache: torch.Tensor, layer_slot_mapping: torch.Tensor):
+        """``do_rope_and_kv_cache_update`` for models that norm each query and
+        key head before the rotation (weights [head_size]), in one launch."""
+        kp, vp = q8_planes(kv_cache, self.num_kv_heads, self.head_size)
+        n = layer_slot_mapping.shape[0]
+        D = self.head_size
+        q = query[:n].view(n, self.num_heads, D)
+        k = key[:n].view(n, self.num_kv_heads, D)
+        v = value[:n].view(n, self.num_kv_heads, D)
+        pos = positions[:n] if positions.dtype == torch.int64 else positions[:n].to(torch.int64)
+        sm = layer_slot_mapping if layer_slot_mapping.dtype == torch.int64 else layer_slot_mapping.to(torch.int64)
+        gfx906_fa.qk_norm_rope_and_cache_q8_kv(pos, q, k, v, query_weight, key_weight, eps, cos_sin_cache, is_neox, sm,
+                                               kp, vp)
+
+    # the score form of every call of the layer (Gfx906FAScoredImpl)
+    soft_cap = 0.0
+
+    def _slopes(self, device: torch.device) -> torch.Tensor | None:
+        return None
+
     @classmethod
     def bound_bytes(cls, heads, limits: tuple[int, int, int]) -> int:
         """The workspace every batch within the scheduler limits needs, plus
@@ -430,18 +473,78 @@ class Gfx906FAImpl(AttentionImpl):
                                 md.max_seq_len, self.head_size)["img_offset"], query.device)
         out = output[:n].view(n, self.num_heads, self.head_size)
         forward_paged(query[:n], kp, vp, md.block_table, md.seq_lens, md.query_start_loc,
-                      md.max_query_len, md.max_seq_len, self.scale, out=out, workspace=ws)
+                      md.max_query_len, md.max_seq_len, self.scale, out=out, workspace=ws,
+                      soft_cap=self.soft_cap, alibi_slopes=self._slopes(query.device),
+                      tree_mask=None if md.tree_mask is None else md.tree_mask[:n])
         return output
+
+
+class Gfx906FAScoredImpl(Gfx906FAImpl):
+    """Layers with a logits soft cap or ALiBi slopes (one of the two); layers
+    with neither are as Gfx906FAImpl's."""
+
+    def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
+                 alibi_slopes: list[float] | None, sliding_window: int | None,
+                 kv_cache_dtype: str, logits_soft_cap: float | None = None,
+                 attn_type: AttentionType = AttentionType.DECODER,
+                 kv_sharing_target_layer_name: int | None = None,
+                 sinks: torch.Tensor | None = None, use_alibi_sqrt: bool = False) -> None:
+        cap = float(logits_soft_cap or 0.0)
+        if use_alibi_sqrt:
+            raise NotImplementedError("GFX906_FA: use_alibi_sqrt is not supported")
+        if cap and alibi_slopes is not None:
+            raise NotImplementedError("GFX906_FA: logits_soft_cap with alibi_slopes is not supported")
+        if not 0.0 <= cap < float("inf"):
+            raise ValueError(f"logits_soft_cap must be positive and finite, got {logits_soft_cap}")
+        if alibi_slopes is not None and len(alibi_slopes) != num_heads:
+            raise ValueError(f"alibi_slopes must have one slope per query head, got {len(alibi_slopes)} for {num_heads}")
+        super().__init__(num_heads, head_size, scale, num_kv_heads, None, sliding_window, kv_cache_dtype, None, attn_type,
+                         kv_sharing_target_layer_name, sinks, False)
+        self.soft_cap = cap
+        self._slope_values = None if alibi_slopes is None else [float(x) for x in alibi_slopes]
+        self._slope_tensors: dict[torch.device, torch.Tensor] = {}
+
+    @classmethod
+    def reserve_workspace(cls, nbytes: int, device: torch.device) -> torch.Tensor:
+        return Gfx906FAImpl.reserve_workspace(nbytes, device)  # one for the layers of both classes
+
+    def _slopes(self, device: torch.device) -> torch.Tensor | None:
+        """The slopes on the layer's device, copied there in its first call (the
+        profiling forward, before any capture)."""
+        if self._slope_values is None:
+            return None
+        t = self._slope_tensors.get(device)
+        if t is None:
+            t = self._slope_tensors[device] = torch.tensor(self._slope_values, dtype=torch.float32, device=device)
+        return t
+
+    def forward(self, layer: torch.nn.Module, query: torch.Tensor, key: torch.Tensor,
+                value: torch.Tensor, kv_cache: torch.Tensor, attn_metadata: Gfx906FAMetadata,
+                output: torch.Tensor | None = None, output_scale: torch.Tensor | None = None,
+                output_block_scale: torch.Tensor | None = None) -> torch.Tensor:
+        if attn_metadata is None and query is not None and query.device.type == "cuda":
+            self._slopes(query.device)
+        return super().forward(layer, query, key, value, kv_cache, attn_metadata, output, output_scale, output_block_scale)
+
+
+class Gfx906FAScoredBackend(Gfx906FABackend):
+    """Gfx906FABackend for models with a logits soft cap or ALiBi."""
+
+    @staticmethod
+    def get_impl_cls() -> type["Gfx906FAImpl"]:
+        return Gfx906FAScoredImpl
 
 
 # -----------------------------------------------------------------------------
 # Registration (reference lines 536-553)
 # -----------------------------------------------------------------------------
 def register() -> None:
-    """Register Gfx906FABackend as AttentionBackendEnum.CUSTOM."""
+    """Register Gfx906FABackend as AttentionBackendEnum.CUSTOM, or with
+    GFX906_FA_SCORES=1 Gfx906FAScoredBackend."""
     from vllm.v1.attention.backends.registry import AttentionBackendEnum, register_backend
 
-    register_backend(AttentionBackendEnum.CUSTOM, f"{__name__}.Gfx906FABackend")
+    name = "Gfx906FAScoredBackend" if os.environ.get("GFX906_FA_SCORES", "0") == "1" else "Gfx906FABackend"
+    register_backend(AttentionBackendEnum.CUSTOM, f"{__name__}.{name}")
     logger.info("GFX906_FA backend registered as AttentionBackendEnum.CUSTOM")
 
 

@@ -119,6 +119,9 @@ def forward_paged(
     *,
     out: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
+    soft_cap: float = 0.0,
+    alibi_slopes: Optional[torch.Tensor] = None,
+    tree_mask: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """vLLM-shaped paged attention; returns ``[num_tokens, Hq*D]``.
 
@@ -127,7 +130,9 @@ def forward_paged(
     is returned like the reference's.  ``key_cache_q8``, ``q_pad_buf``,
     ``mask_buf``, ``k_gather_buf`` and ``v_gather_buf`` are accepted for call
     compatibility with the reference and unused: nothing is padded or
-    gathered.  ``key_cache_q8``, if given, must be ``key_cache``."""
+    gathered.  ``key_cache_q8``, if given, must be ``key_cache``.
+    ``soft_cap``, ``alibi_slopes`` and ``tree_mask`` select
+    ``gfx906_fa.scored_paged_attention`` or ``gfx906_fa.tree_attention``."""
     if key_cache_q8 is not None and key_cache_q8.data_ptr() != key_cache.data_ptr():
         raise RuntimeError("key_cache_q8 must alias key_cache (K is always Q8_0 here)")
     num_tokens, Hq, D = query.shape
@@ -149,9 +154,17 @@ def forward_paged(
         if query.is_cuda:
             torch.cuda.synchronize(query.device)
     try:
-        res = gfx906_fa.paged_attention(query, key_cache, value_cache, bt, sl.contiguous(), cu.contiguous(),
-                                        max_seqlen_q, max_seqlen_k, scale, out=o3, workspace=workspace,
-                                        out_dtype=torch.float32)
+        args = (query, key_cache, value_cache, bt, sl.contiguous(), cu.contiguous())
+        more = dict(out=o3, workspace=workspace, out_dtype=torch.float32)
+        if tree_mask is not None:
+            if alibi_slopes is not None:
+                raise RuntimeError("tree_mask and alibi_slopes exclude each other")
+            res = gfx906_fa.tree_attention(*args, tree_mask, max_seqlen_q, max_seqlen_k, scale, soft_cap=soft_cap, **more)
+        elif soft_cap or alibi_slopes is not None:
+            res = gfx906_fa.scored_paged_attention(*args, max_seqlen_q, max_seqlen_k, scale, soft_cap=soft_cap,
+                                                   alibi_slopes=alibi_slopes, **more)
+        else:
+            res = gfx906_fa.paged_attention(*args, max_seqlen_q, max_seqlen_k, scale, **more)
         if _DBG:
             if query.is_cuda:
                 torch.cuda.synchronize(query.device)

@@ -117,3 +117,28 @@ def test_custom_ops():
         assert o.shape == q.shape and o.dtype == torch.bfloat16
         k, v = OPS.read_cache_q8_kv(e((7,), torch.int64), c[:, 0], c[:, 1], torch.float16)
         assert k.shape == v.shape == (7, 2, 128) and k.dtype == torch.float16
+
+
+def test_backend_takes_the_score_forms(monkeypatch):
+    import gfx906_fa_backend as B
+    args = dict(num_heads=8, head_size=128, scale=0.1, num_kv_heads=1, alibi_slopes=None, sliding_window=None,
+                kv_cache_dtype="auto")
+    assert B.Gfx906FAScoredBackend.get_impl_cls() is B.Gfx906FAScoredImpl
+    assert B.Gfx906FAScoredImpl(**args, logits_soft_cap=30.0).soft_cap == 30.0
+    impl = B.Gfx906FAScoredImpl(**{**args, "alibi_slopes": [0.5] * 8})
+    assert impl._slopes(torch.device("cpu")).tolist() == [0.5] * 8 and impl.soft_cap == 0.0
+    assert B.Gfx906FAScoredImpl(**args)._slopes(torch.device("cpu")) is None
+    for err, kw in ((ValueError, dict(alibi_slopes=[0.5])), (ValueError, dict(logits_soft_cap=-1.0)),
+                    (ValueError, dict(logits_soft_cap=float("inf"))),
+                    (NotImplementedError, dict(logits_soft_cap=2.0, alibi_slopes=[0.5] * 8)),
+                    (NotImplementedError, dict(sliding_window=64)), (NotImplementedError, dict(use_alibi_sqrt=True)),
+                    (NotImplementedError, dict(sinks=torch.zeros(8)))):
+        with pytest.raises(err):
+            B.Gfx906FAScoredImpl(**{**args, **kw})
+    names = []
+    import vllm.v1.attention.backends.registry as R
+    monkeypatch.setattr(R, "register_backend", lambda where, name: names.append(name))
+    B.register()
+    monkeypatch.setenv("GFX906_FA_SCORES", "1")
+    B.register()
+    assert [n.rsplit(".", 1)[1] for n in names] == ["Gfx906FABackend", "Gfx906FAScoredBackend"]

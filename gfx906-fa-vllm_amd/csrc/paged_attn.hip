@@ -167,8 +167,9 @@ struct AttnParams {
 constexpr int SC_NONE = 0, SC_TREE = 1, SC_CAP = 2, SC_BIAS = 3;
 
 // cap * tanh(s / cap) in log2 units, from x = 2 log2 e * s / cap: with t = 2^x,
-// tanh = 1 - 2 / (1 + t), exact at both ends (t = 0, inf) and within 2e-7 * cap
-// of it between.  less: subtracted from the result (a running max).
+// tanh = 1 - 2 / (1 + t), exact at both ends (t = 0, inf) and within 1.2e-7 * cap
+// of it between: at the largest cap taken, 1024, a quarter of fp16's half step.
+// less: subtracted from the result (a running max).
 __device__ __forceinline__ float capped(float x, float cap_log2e, float less) {
     return fmaf(-2.0f * cap_log2e, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), cap_log2e - less);
 }
@@ -3586,10 +3587,14 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // [0.5, 1): K^ = fp16(q * d_k * kmul) stays at or below the dequantized key
 // q * d_k, so it is finite wherever the decode kernel's fp16(q * d_k) is
 // (a kmul up to 2 would overflow keys above 65504 / kmul, 32.8K at worst).
-void set_prefill_scale(AttnParams &p) {
+// Capped scores carry 2 log2 e * scale / cap instead, far below 1 for the usual
+// caps: below 2^-8 K^ takes the rest (its ints times a scale near 1 / 127 of
+// the keys keep their bits down to 2^-7 of that).
+void set_prefill_scale(AttnParams &p, bool capped) {
     int e = 0;
     (void)frexpf(p.scale_log2e, &e);  // c = m * 2^e, m in [0.5, 1)
     e = max(-60, min(60, -e));
+    if (capped) e = min(e, 8);
     p.pf_qmul = ldexpf(1.0f, -e);
     p.pf_kmul = ldexpf(p.scale_log2e, e);
 }
@@ -4147,7 +4152,7 @@ hipError_t paged_attention_impl(
     p.cap_log2e = scores ? scores->cap * LOG2E : 0.0f;
     p.slopes = scores ? scores->slopes : nullptr;
     p.tree = scores ? scores->tree : nullptr;
-    set_prefill_scale(p);
+    set_prefill_scale(p, p.cap_log2e > 0.0f);
     set_divisors(p);
     p.out = out;
     p.o_ts = out_token_stride;
@@ -4312,10 +4317,11 @@ extern "C" hipError_t gfx906_fa_amd_scored_paged_attention(
     int block_size, int max_query_len, int max_seq_len, float scale, void *out, int out_dtype,
     int64_t out_token_stride, int64_t out_head_stride, void *workspace, size_t workspace_bytes,
     hipStream_t stream) {
-    if (!(soft_cap >= 0.0f) || (soft_cap > 0.0f && !std::isfinite(scale * (2.0f * LOG2E / soft_cap))) ||
-        !std::isfinite(soft_cap * LOG2E)) {
-        fprintf(stderr, "[gfx906_fa_amd] scored_paged_attention: soft_cap must be 0 or positive, finite and no "
-                        "smaller than the scale allows (got %g)\n", (double)soft_cap);
+    // (the ratio bounds what the prefill kernel's fp16 Q and K^ carry: 2^-14 to 2^6)
+    const float ratio = fabsf(scale) * 32768.0f / soft_cap;
+    if (!(soft_cap >= 0.0f && soft_cap <= 1024.0f) || (soft_cap > 0.0f && !(ratio >= 1.0f && ratio <= 1048576.0f))) {
+        fprintf(stderr, "[gfx906_fa_amd] scored_paged_attention: soft_cap must be 0 (none), or positive, at most 1024 and "
+                        "1/32 to 32768 times the scale (got %g, scale %g)\n", (double)soft_cap, (double)scale);
         return hipErrorInvalidValue;
     }
     if (alibi_slopes && (soft_cap > 0.0f || tree_mask)) {
@@ -4515,7 +4521,7 @@ extern "C" hipError_t gfx906_fa_amd_flat_attention(
     p.G = G;
     p.block_size = 16;
     p.scale_log2e = scale * LOG2E;
-    set_prefill_scale(p);
+    set_prefill_scale(p, false);
     set_divisors(p);
     p.out = out;
     p.num_seqs = batch;
@@ -4597,7 +4603,7 @@ extern "C" hipError_t gfx906_fa_amd_paged_attention_tiled(
     p.G = num_heads / num_kv_heads;
     p.block_size = block_size;
     p.scale_log2e = scale * LOG2E;
-    set_prefill_scale(p);
+    set_prefill_scale(p, false);
     set_divisors(p);
     p.out = out;
     p.o_ts = out_token_stride;

@@ -348,6 +348,7 @@ __device__ __forceinline__ void store_row_chunk(const RopeArgs &a, int64_t slot,
 struct NormArgs {
     RopeArgs r;
     const void *wq, *wk;
+    int64_t num_slots;  // slots of the cache: others are not written
     float eps;
 };
 
@@ -500,7 +501,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
         uint32_t klo, khi, vlo, vhi;
         const float dk = quant8(x, klo, khi);
         const float dv = quant8(vv, vlo, vhi);
-        if (slot < 0) continue;
+        if (slot < 0 || slot >= n.num_slots) continue;
         store_row_chunk(a, slot, row - a.Hq, i, klo, khi, dk, vlo, vhi, dv);
     }
 }
@@ -640,7 +641,7 @@ extern "C" hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
     float eps, int dtype, const int64_t *positions,
     const void *cos_sin_cache, int cos_sin_dtype, int64_t cos_sin_stride, int max_position,
     int rot_dim, int is_neox, const int64_t *slot_mapping, uint8_t *k_cache, uint8_t *v_cache,
-    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
     int64_t query_token_stride, int64_t query_head_stride, int64_t key_token_stride,
     int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
     int64_t cache_block_stride, int64_t cache_head_stride, hipStream_t stream) {
@@ -660,6 +661,7 @@ extern "C" hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
     if (grid == 0) return hipSuccess;
     a.wq = query_weight;
     a.wk = key_weight;
+    a.num_slots = num_blocks * block_size;
     a.eps = eps;
     const bool neox = is_neox != 0;
 #define GFA_NORM_CS(DT)                                                     \

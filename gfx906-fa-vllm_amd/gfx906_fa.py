@@ -109,7 +109,7 @@ def _load():
         "gfx906_fa_amd_scored_paged_attention": (I, [P, I, I64, I64, P, P, I64, I64, P, I64, P, P, P, I, F, P, P,
                                                      I, I, I, I, I, I, I, I, F, P, I, I64, I64, P, SZ, P]),
         "gfx906_fa_amd_qk_norm_rope_cache_write_kv": (I, [P, P, P, P, P, F, I, P, P, I, I64, I, I, I, P, P, P,
-                                                          I, I, I, I, I, I64, I64, I64, I64, I64, I64, I64, I64, P]),
+                                                          I, I, I, I, I, I64, I64, I64, I64, I64, I64, I64, I64, I64, P]),
         "gfx906_fa_amd_read_rows": (I, [P, P, P, P, P, I, I64, I, I, I, I64, I64, I64, I64, I64, I64, I64, P]),
         "gfx906_fa_amd_compact_draft_rows": (I, [P, P, P, P, I64, I, I64, I64, I64, P, I64, I, P, P, P, I64, I, P,
                                                  I, I, I, I, P]),
@@ -611,6 +611,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
 # Scored and tree attention, norms with rotation, draft rows
 # ---------------------------------------------------------------------------
 MAX_TREE_NODES = 64
+MAX_SOFT_CAP = 1024.0  # the fp32 tanh's error grows with the cap
 
 
 _get_device = torch._C._cuda_getDevice
@@ -651,8 +652,8 @@ def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_lo
         raise RuntimeError("query must be [num_tokens, Hq, 128]")
     T, Hq, D = shape
     soft_cap = float(soft_cap)
-    if not 0.0 <= soft_cap < float("inf"):
-        raise RuntimeError(f"soft_cap must be 0 (none) or positive and finite, got {soft_cap}")
+    if not 0.0 <= soft_cap <= MAX_SOFT_CAP:
+        raise RuntimeError(f"soft_cap must be 0 (none) or positive, at most {MAX_SOFT_CAP:g}, got {soft_cap}")
     if alibi_slopes is not None:
         if soft_cap > 0.0:
             raise RuntimeError("soft_cap and alibi_slopes exclude each other")
@@ -727,7 +728,8 @@ def scored_paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
                            causal: bool = True, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``paged_attention`` with another score.  With s = scale * q.k:
 
-    ``soft_cap`` > 0: cap * tanh(s / cap).
+    ``soft_cap`` > 0 (at most 1024, and 1/32 to 32768 times the scale):
+    cap * tanh(s / cap).
     ``alibi_slopes`` (fp32 [Hq]): s + slope[head] * (key position - row
     position); row j of a sequence is at position seq_len - n_q + j, or at
     q_abs_offset + j.  Rows of causal batches see no later key, so a positive
@@ -786,7 +788,7 @@ def qk_norm_rope_and_cache_q8_kv(positions: torch.Tensor, query: torch.Tensor, k
     x * rsqrt(mean(x^2) + eps) * weight (``query_weight`` / ``key_weight`` [128],
     the model dtype), then its first rot_dim values are rotated, in place, in
     fp32 and rounded once; the stored key and the value go to the cache as Q8_0
-    at slot_mapping (< 0 skips).  One launch.  Rows at positions outside
+    at slot_mapping (slots outside the cache, < 0 too, are skipped).  One launch.  Rows at positions outside
     [0, max_position) are normed and not rotated."""
     at = query.get_device()
     if at < 0:
@@ -845,8 +847,8 @@ def qk_norm_rope_and_cache_q8_kv(positions: torch.Tensor, query: torch.Tensor, k
     err = _lib.gfx906_fa_amd_qk_norm_rope_cache_write_kv(
         query.data_ptr(), key.data_ptr(), value.data_ptr(), query_weight.data_ptr(), key_weight.data_ptr(), float(eps), qdt,
         positions.data_ptr(), cos_sin_cache.data_ptr(), cdt, cos_sin_cache.stride(0), npos, rot, 1 if is_neox else 0,
-        slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), T, Hq, Hkv, D, bs, qts, qhs, kts, khs, vts,
-        vhs, cbs, chs, _stream(query.device))
+        slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), T, Hq, Hkv, D, bs, key_cache.shape[0], qts,
+        qhs, kts, khs, vts, vhs, cbs, chs, _stream(query.device))
     if err:
         _ok(err, "gfx906_fa_amd_qk_norm_rope_cache_write_kv")
 

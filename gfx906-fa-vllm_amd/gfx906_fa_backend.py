@@ -494,8 +494,8 @@ class Gfx906FAScoredImpl(Gfx906FAImpl):
             raise NotImplementedError("GFX906_FA: use_alibi_sqrt is not supported")
         if cap and alibi_slopes is not None:
             raise NotImplementedError("GFX906_FA: logits_soft_cap with alibi_slopes is not supported")
-        if not 0.0 <= cap < float("inf"):
-            raise ValueError(f"logits_soft_cap must be positive and finite, got {logits_soft_cap}")
+        if not 0.0 <= cap <= gfx906_fa.MAX_SOFT_CAP:
+            raise ValueError(f"logits_soft_cap must be positive, at most {gfx906_fa.MAX_SOFT_CAP:g}, got {logits_soft_cap}")
         if alibi_slopes is not None and len(alibi_slopes) != num_heads:
             raise ValueError(f"alibi_slopes must have one slope per query head, got {len(alibi_slopes)} for {num_heads}")
         super().__init__(num_heads, head_size, scale, num_kv_heads, None, sliding_window, kv_cache_dtype, None, attn_type,

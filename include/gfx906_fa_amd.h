@@ -457,7 +457,8 @@ hipError_t gfx906_fa_amd_paged_attention_padded(
     float *out, void *workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* (11) Scored paged attention: (5) with another score.  With s = scale * q.k
- *     soft_cap > 0:   cap * tanh(s / cap)
+ *     soft_cap > 0:   cap * tanh(s / cap), cap at most 1024 and 1/32 to
+ *                     32768 times the scale
  *     alibi_slopes:   s + slopes[head] * (key position - row position); fp32
  *                     [num_heads], row j at position seq_len - n_q + j (or
  *                     q_abs_offset + j)
@@ -488,13 +489,14 @@ hipError_t gfx906_fa_amd_scored_paged_attention(
  *     (query_weight, key_weight: [128] of the model dtype, 16-byte aligned),
  *     then the rotary pairs, in fp32 and rounded once to the model dtype as
  *     query and key are stored in place.  The cache takes the stored key.
- *     Positions outside [0, max_position) are normed and not rotated. */
+ *     Positions outside [0, max_position) are normed and not rotated; slots
+ *     outside the cache of num_blocks pages are not written. */
 hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
     void *query, void *key, const void *value, const void *query_weight, const void *key_weight,
     float eps, int dtype, const int64_t *positions,
     const void *cos_sin_cache, int cos_sin_dtype, int64_t cos_sin_stride, int max_position,
     int rot_dim, int is_neox, const int64_t *slot_mapping, uint8_t *k_cache, uint8_t *v_cache,
-    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size,
+    int num_tokens, int num_heads, int num_kv_heads, int head_size, int block_size, int64_t num_blocks,
     int64_t query_token_stride, int64_t query_head_stride, int64_t key_token_stride,
     int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride,
     int64_t cache_block_stride, int64_t cache_head_stride, hipStream_t stream);

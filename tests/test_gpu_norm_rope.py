@@ -58,6 +58,7 @@ def _run(dt, T, Hq, Hkv, rot, neox, cs_dtype, bs=16, seed=0, eps=1e-6, spread=2.
     if edges and T > 8:
         pos[2], pos[5], pos[7] = -1, cs.shape[0], 0
         slots[1] = slots[T - 1] = -1
+        slots[4] = NB * bs  # past the cache: not written
     q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:]  # views of one projection
     q0, k0, v0 = (t.clone() for t in (q, k, v))
     cache = torch.full((NB, 2, Hkv, bs // 16 * 2176), 0x5A, dtype=torch.uint8, device=DEV)
@@ -68,7 +69,7 @@ def _run(dt, T, Hq, Hkv, rot, neox, cs_dtype, bs=16, seed=0, eps=1e-6, spread=2.
     _assert_rows(k, *_ref(k0, wk, eps, pos, cs, rot, neox))
     assert torch.equal(v, v0)
     exp = np.full(tuple(cache.shape), 0x5A, np.uint8)
-    O.planar_cache_write(host_bits(k.contiguous()), host_bits(v0), slots.numpy(), exp)
+    O.planar_cache_write(host_bits(k.contiguous()), host_bits(v0), np.where(slots.numpy() < NB * bs, slots.numpy(), -1), exp)
     assert np.array_equal(cache.cpu().numpy(), exp)
 
 

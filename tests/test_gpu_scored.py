@@ -30,6 +30,7 @@ SHAPES = {
     "chunk_split": ([2100], [50], 6, 1, 32),
     "mixed": ([90, 640, 1, 333, 64], [90, 1, 1, 20, 5], 6, 1, 16),
     "mixed_wide": ([200, 90, 700], [1, 1, 3], 20, 1, 16),
+    "images": ([1400], [1400], 6, 1, 16),   # 33 row tiles: key tiles dequantized once
 }
 
 
@@ -75,7 +76,7 @@ def test_biased(name, dt):
     check(out, *scored_oracle(b, slopes=sl.cpu().numpy()))
 
 
-@pytest.mark.parametrize("cap", [0.01, 1.0, 30.0, 1e4])
+@pytest.mark.parametrize("cap", [0.003, 1.0, 30.0, 1024.0])
 @pytest.mark.parametrize("name", ["decode", "prompts"])
 def test_cap_range(name, cap):
     """From a cap that flattens every score to one that changes none."""
@@ -120,6 +121,18 @@ def test_visibility(name, form, how):
     check(out, ref, bound)
     if how == "hidden":
         assert (np.abs(ref).max(axis=(1, 2)) == 0).any()
+
+
+@pytest.mark.parametrize("scale", [1e-4, 4.0])
+@pytest.mark.parametrize("name", ["decode", "prompts"])
+def test_scale_range(name, scale):
+    """Scales far from 1 / sqrt(128) with a cap of the scores' size."""
+    need_gpu()
+    announce(f"scale {scale} {name}")
+    b = _batch(name, "bf16", spread=0.05 / scale if scale < 1 else 0.2)
+    b.scale = scale
+    out = _call(b, soft_cap=2.0, out_dtype=torch.float32)
+    check(out, *scored_oracle(b, cap=2.0))
 
 
 def test_no_form_is_plain_attention():
@@ -206,7 +219,7 @@ def test_refusals():
     announce("refusals")
     b = _batch("decode", "f16", poison=False)
     sl = _slopes(b.Hq)
-    for kw in (dict(soft_cap=-1.0), dict(soft_cap=float("nan")), dict(soft_cap=float("inf")), dict(soft_cap=1e-44),
+    for kw in (dict(soft_cap=-1.0), dict(soft_cap=float("nan")), dict(soft_cap=float("inf")), dict(soft_cap=1e-44), dict(soft_cap=1e-4), dict(soft_cap=1025.0),
                dict(soft_cap=2.0, alibi_slopes=sl), dict(alibi_slopes=sl[:-1]), dict(alibi_slopes=sl.half()),
                dict(alibi_slopes=sl.cpu()), dict(soft_cap=2.0, out_dtype=torch.bfloat16),
                dict(soft_cap=2.0, out=torch.empty(4, 48, 128, dtype=torch.bfloat16, device=DEV)),

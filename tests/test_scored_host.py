@@ -44,7 +44,7 @@ def _scored(**kw):
 def test_scored_entry_refusals():
     p = ctypes.c_void_p(256)
     assert _scored(T=0, cap=5.0) == 0
-    for kw in (dict(cap=-1.0), dict(cap=float("nan")), dict(cap=float("inf")), dict(cap=1e-44), dict(cap=2.0, slopes=p),
+    for kw in (dict(cap=-1.0), dict(cap=float("nan")), dict(cap=float("inf")), dict(cap=1e-44), dict(cap=1025.0), dict(cap=0.003), dict(cap=1.0, scale=1e-5), dict(cap=1.0, scale=float("nan")), dict(cap=2.0, slopes=p),
                dict(slopes=p, tree=p), dict(tree=p, mq=65), dict(tree=p, qa=p), dict(tree=p, causal=0),
                dict(cap=2.0, qdt=0, odt=0), dict(cap=2.0, qdt=1, odt=2), dict(cap=2.0, qdt=2, odt=1), dict(cap=2.0, D=64),
                dict(cap=2.0, bs=24), dict(cap=2.0, Hq=9, Hkv=2), dict(cap=2.0, wsb=128)):
@@ -54,7 +54,7 @@ def test_scored_entry_refusals():
 def test_norm_rope_entry_refusals():
     f = gfx906_fa.lib().gfx906_fa_amd_qk_norm_rope_cache_write_kv
     good = [None, None, None, None, None, 1e-6, 1, None, None, 1, 128, 4096, 128, 1, None, None, None, 0, 8, 2, 128, 16,
-            0, 0, 0, 0, 0, 0, 0, 0, None]
+            4, 0, 0, 0, 0, 0, 0, 0, 0, None]
     assert f(*good) == 0
     for at, value in ((3, ctypes.c_void_p(8)), (4, ctypes.c_void_p(2)), (5, -1.0), (5, float("nan")), (6, 0), (12, 72),
                       (12, 256), (20, 64), (21, 24)):

@@ -153,6 +153,8 @@ struct AttnParams {
     // cap_log2e = cap * log2 e, and scale_log2e (and with it pf_qmul * pf_kmul)
     // is 2 * log2 e * scale / cap.  SC_BIAS: one slope per query head.  tree
     // (SC_TREE; SC_CAP where given): a 64-bit mask per query row.
+    // whole: a decode launch of short contexts, every segment one piece (no merge).
+    int whole;
     float cap_log2e;
     const float *slopes;
     const int64_t *tree;
@@ -1112,6 +1114,9 @@ __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void at
             // what stream-K would give each workgroup, and a little
             const float even = 16.0f * (float)tot / (float)maxc;
             int upw = max((int)ceilf(even), 16 * GFA_DEC_ALIGN_UNITS);
+            if constexpr (SC != SC_NONE) {
+                if (p.whole) upw = 1 << 20;  // (the host has checked nseg <= maxc)
+            }
             for (int t = 0; t < 2 && d.upw == 0; ++t) {
                 lc = ln > 0 ? pl_div(16 * ln + upw - 1, upw) : 0;
                 cincl = wave_incl_scan(lc);
@@ -3569,6 +3574,7 @@ struct Plan {
     size_t list_extra;  // bytes of the work list past 20 an item (see the allocation-free entry)
     size_t bytes;       // the regions a call needs; the tile images follow at `bytes`
     size_t img_bytes;   // room the tile images of the call's shape can take (capped)
+    int64_t max_seq_len;
     bool comb_short;    // contexts of at most GFA_COMB_FEW_KEYS keys (combine choice)
 };
 
@@ -3765,6 +3771,7 @@ Plan make_plan(int num_seqs, int num_tokens, int num_heads, int num_kv_heads, in
     pl.pf_rows = max_rows <= GFA_PF_KS2_MAX_ROWS ? PF_ROWS / 2 : PF_ROWS;
     plan_finish(pl, num_seqs, num_tokens, G, num_kv_heads, false, allow_split, max_seq_len, max_query_len);
     pl.comb_short = max_seq_len <= GFA_COMB_FEW_KEYS;
+    pl.max_seq_len = max_seq_len;
     return pl;
 }
 
@@ -3849,6 +3856,21 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
         pd.ws_pre = reinterpret_cast<int *>(ws + c.off_pre);
         pd.ws_ml = reinterpret_cast<float *>(ws + c.off_ml);
         pd.ws_o = reinterpret_cast<float *>(ws + c.off_o);
+        bool merge = true;
+        if constexpr (SC != SC_NONE) {
+            // Short contexts: splitting a segment saves less than its merge costs.
+            // Measured from graphs, fp16, capped (whole against split): one row
+            // group, 1 x 384 keys 9.3 and 9.9 us, 1 x 512 10.8 and 9.9; 30 rows,
+            // 1 x 384 12.8 and 13.2, 1 x 512 14.3 and 13.1; 48 to 64 rows, 1 x 128
+            // 12.1 and 14.0, 1 x 256 16.0 and 14.9.  With a segment per CU and
+            // more (32 sequences): 256 x 1024 at 48/8 18.0 and 20.8, 64 rows 49.9
+            // and 61.4.
+            const bool wide = c.nrg == 3 || (c.nrg == 2 && c.rows_hi > 32);
+            const int64_t most = (int64_t)num_seqs * num_kv_heads >= device_cus() ? 1024 : wide ? 128 : 384;
+            const int wgs = c.nrg == 2 && !wide ? c.nwg * DEC_NW / dec_nw(2, false) : c.nwg;
+            pd.whole = num_seqs <= min(64, wgs / num_kv_heads) && pl.max_seq_len <= most;
+            merge = !pd.whole;
+        }
         // combine rows: a split segment has at most min(max_query_len * G, slot) rows
         const int crow = max(1, min(max_query_len * p.G, c.rows_hi));
         if (c.nrg == 1) {
@@ -3858,13 +3880,14 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
             // There the merge launch is mostly workgroups that find their
             // segment whole (32 x 32 keys, 48/8: 6.7 against 7.9 us per
             // call); with long contexts the per-row launch measured faster.
+            if (!merge) continue;
             if (pl.comb_short && (int64_t)c.nwg <= (int64_t)GFA_COMB_FEW * num_seqs * num_kv_heads)
                 attn_combine_few_kernel<ODT><<<dim3(num_seqs, num_kv_heads), 256, 0, stream>>>(pd);
             else
                 attn_combine_kernel<1, ODT><<<dim3(num_seqs, num_kv_heads, crow), 256, 0, stream>>>(pd);
         } else if (c.nrg == 3) {
             attn_decode_kernel<3, QDT, ODT, false, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
-            attn_combine_kernel<3, ODT><<<dim3(num_seqs, num_kv_heads, crow), 256, 0, stream>>>(pd);
+            if (merge) attn_combine_kernel<3, ODT><<<dim3(num_seqs, num_kv_heads, crow), 256, 0, stream>>>(pd);
         } else {
             if (c.rows_hi > 32) attn_decode_kernel<2, QDT, ODT, true, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
             else {  // one 8-wave workgroup where the plan sized two 4-wave ones
@@ -3874,6 +3897,7 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
             }
             // (a mixed batch's class mostly finds nothing to merge: 250 prompts
             // of 30 tokens at 48/8 128 us with a launch per row, 89.5 per segment)
+            if (!merge) continue;
             if ((c.rows_lo > 0 || pl.one_class) && (int64_t)num_seqs * num_kv_heads >= GFA_COMB_SEGS)
                 attn_combine_few_kernel<ODT><<<dim3(num_seqs, num_kv_heads), 256, 0, stream>>>(pd);
             else
@@ -4177,6 +4201,7 @@ hipError_t paged_attention_impl(
     p.ws_ml = nullptr;
     p.ws_o = nullptr;
     p.nwg = 0;
+    p.whole = 0;
     p.new_k = p.new_v = nullptr;
     p.nk_ts = p.nk_hs = p.nv_ts = p.nv_hs = 0;
     p.new_slot = nullptr;

@@ -24,6 +24,10 @@ SHAPES = {
     "verify30": ([640, 35, 5], [5, 5, 5], 6, 1, 16),
     "verify48_tiles": ([1040] * 8, [8] * 8, 48, 8, 16),
     "verify64": ([300, 8], [8, 8], 8, 1, 16),
+    "verify64_short": ([100, 70, 8], [8, 8, 8], 8, 1, 16),
+    "verify30_short": ([384, 71, 6], [5, 5, 5], 6, 1, 16),
+    "many_short": ([1024] + [100] * 31, [1] * 32, 32, 8, 16),
+    "many_verify": ([200] * 16 + [9] * 16, [5] * 32, 48, 8, 16),
     "rows96": ([700, 12], [12, 12], 8, 1, 16),
     "rows360": ([500], [60], 48, 8, 16),
     "prompts": ([77, 301, 130], [77, 301, 130], 8, 2, 16),

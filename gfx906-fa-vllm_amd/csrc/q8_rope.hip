@@ -395,6 +395,10 @@ __device__ __forceinline__ void load_cs_f32(const void *row, int col, float (&v)
     for (int e = 0; e < N; e += 2) load2_as_f32<CSDT>(row, col + e, v[e], v[e + 1]);
 }
 
+// Rows per wave: 4 x 4, or 4 x 2 below NORM_FEW_WAVES waves of 32 rows, so that
+// more waves share few tokens (64 tokens at 48/8: 5.9 us with 32 rows a wave,
+// 5.0 with 8; 8192 tokens: 68.4 us with 32, 66.2 with 16, 73.2 with 8).
+constexpr int NORM_ITERS = 4, NORM_FEW_ITERS = 2;
 #ifndef GFA_NORM_FEW_WAVES
 #define GFA_NORM_FEW_WAVES 2048
 #endif
@@ -403,7 +407,25 @@ constexpr int NORM_FEW_WAVES = GFA_NORM_FEW_WAVES;
 template <int DT, int CSDT, bool NEOX, int ITERS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q8_norm_rope_cache_write_kernel(NormArgs n) {
     const RopeArgs &a = n.r;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Many tokens stream through once, more than the caches hold for the
+    // attention to find: nontemporal both ways (8192 tokens at 48/8, bf16, 66.5
+    // -> 59.7 us, 4.55 TB/s; loads alone 63.7, stores alone 64.9).
+    constexpr bool NT = ITERS > 2;
+    auto load = [](const uint16_t *p) __attribute__((always_inline)) {
+        const u32x4_t *v = reinterpret_cast<const u32x4_t *>(p);
+        if constexpr (NT) return __builtin_nontemporal_load(v);
+        else return *v;
+    };
+    // Consecutive workgroups go to the eight XCDs in turn: within runs of 8
+    // times the workgroups of 16 tokens, each XCD takes 16 tokens that follow
+    // each other, so that a sub-page's lines fill up in one L2 instead of going
+    // out in parts from eight (8192 tokens 70.5 -> 68.4 us).
+    int block = blockIdx.x;
+    {
+        const int g = 4 * a.nchunk, first = block - block % (8 * g), r = block - first;
+        if (first + 8 * g <= (int)gridDim.x) block = first + (r & 7) * g + (r >> 3);
+    }
+    const int64_t wave = (int64_t)block * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
     const int d0 = 8 * i;
@@ -418,14 +440,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
         vw[it] = u32x4_t{0, 0, 0, 0};
         const int row = c0 + 4 * it + g;
         if (row < a.Hq) {
-            xw[it] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(a.q) + t * a.qts +
-                                                      (int64_t)row * a.qhs + d0);
+            xw[it] = load(static_cast<const uint16_t *>(a.q) + t * a.qts + (int64_t)row * a.qhs + d0);
         } else if (row < R) {
             const int h = row - a.Hq;
-            xw[it] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(a.k) + t * a.kts +
-                                                      (int64_t)h * a.khs + d0);
-            vw[it] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(a.v) + t * a.vts +
-                                                      (int64_t)h * a.vhs + d0);
+            xw[it] = load(static_cast<const uint16_t *>(a.k) + t * a.kts + (int64_t)h * a.khs + d0);
+            vw[it] = load(static_cast<const uint16_t *>(a.v) + t * a.vts + (int64_t)h * a.vhs + d0);
         }
     }
     const int64_t pos = a.pos[t];
@@ -488,7 +507,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
         if (!active) continue;
         uint16_t *dst = is_q ? static_cast<uint16_t *>(a.q) + t * a.qts + (int64_t)row * a.qhs + d0
                              : static_cast<uint16_t *>(a.k) + t * a.kts + (int64_t)(row - a.Hq) * a.khs + d0;
-        *reinterpret_cast<u32x4_t *>(dst) = w;
+        if constexpr (NT) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t *>(dst));
+        else *reinterpret_cast<u32x4_t *>(dst) = w;
         if (is_q) continue;
         float vv[8];
 #pragma unroll
@@ -507,21 +527,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
 }
 
 template <int DT, int CSDT>
-void launch_norm_rope(const NormArgs &a, bool neox, hipStream_t stream) {
+hipError_t launch_norm_rope(const NormArgs &a, bool neox, hipStream_t stream) {
     NormArgs n = a;
     const int rows = a.r.Hq + a.r.Hkv;
-    // few tokens: 8 rows a wave instead of 32, so that more waves share them
     const bool few = a.r.num_tokens * ((rows + 31) / 32) < NORM_FEW_WAVES;
-    const int per = 4 * (few ? 2 : ROPE_ITERS);
+    const int per = 4 * (few ? NORM_FEW_ITERS : NORM_ITERS);
     n.r.nchunk = (rows + per - 1) / per;
-    const unsigned grid = (unsigned)((a.r.num_tokens * n.r.nchunk + 3) / 4);
-    if (few) {
-        if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true, 2><<<grid, 256, 0, stream>>>(n);
-        else q8_norm_rope_cache_write_kernel<DT, CSDT, false, 2><<<grid, 256, 0, stream>>>(n);
-    } else {
-        if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true, ROPE_ITERS><<<grid, 256, 0, stream>>>(n);
-        else q8_norm_rope_cache_write_kernel<DT, CSDT, false, ROPE_ITERS><<<grid, 256, 0, stream>>>(n);
+    const int64_t blocks = (a.r.num_tokens * n.r.nchunk + 3) / 4;
+    if (blocks > 0x7FFFFFFF) {
+        fprintf(stderr, "[gfx906_fa_amd] qk_norm_rope_cache_write_kv: too many rows\n");
+        return hipErrorInvalidValue;
     }
+    const unsigned grid = (unsigned)blocks;
+    if (few) {
+        if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true, NORM_FEW_ITERS><<<grid, 256, 0, stream>>>(n);
+        else q8_norm_rope_cache_write_kernel<DT, CSDT, false, NORM_FEW_ITERS><<<grid, 256, 0, stream>>>(n);
+    } else {
+        if (neox) q8_norm_rope_cache_write_kernel<DT, CSDT, true, NORM_ITERS><<<grid, 256, 0, stream>>>(n);
+        else q8_norm_rope_cache_write_kernel<DT, CSDT, false, NORM_ITERS><<<grid, 256, 0, stream>>>(n);
+    }
+    return hipGetLastError();
 }
 
 // Checks an entry's arguments and fills in the kernel's; grid 0: nothing to do.
@@ -666,9 +691,9 @@ extern "C" hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
     const bool neox = is_neox != 0;
 #define GFA_NORM_CS(DT)                                                     \
     switch (cos_sin_dtype) {                                                \
-        case GFA_DTYPE_F32: launch_norm_rope<DT, GFA_DTYPE_F32>(a, neox, stream); break; \
-        case GFA_DTYPE_F16: launch_norm_rope<DT, GFA_DTYPE_F16>(a, neox, stream); break; \
-        default: launch_norm_rope<DT, GFA_DTYPE_BF16>(a, neox, stream); break;           \
+        case GFA_DTYPE_F32: return launch_norm_rope<DT, GFA_DTYPE_F32>(a, neox, stream); \
+        case GFA_DTYPE_F16: return launch_norm_rope<DT, GFA_DTYPE_F16>(a, neox, stream); \
+        default: return launch_norm_rope<DT, GFA_DTYPE_BF16>(a, neox, stream);           \
     }
     if (dtype == GFA_DTYPE_F16) {
         GFA_NORM_CS(GFA_DTYPE_F16)
@@ -676,5 +701,4 @@ extern "C" hipError_t gfx906_fa_amd_qk_norm_rope_cache_write_kv(
         GFA_NORM_CS(GFA_DTYPE_BF16)
     }
 #undef GFA_NORM_CS
-    return hipGetLastError();
 }

@@ -32,6 +32,9 @@
 //                        32-row chunks
 //   attn_prefill_kernel  sequences with more rows: 128-row workgroups share
 //                        K/V tiles dequantized to fp16 in LDS; 32x32x16 MFMA
+//
+// Both also in scored forms (their SC parameter): scores capped by a tanh,
+// biased by the distance, or of a tree of drafted tokens.
 #include <atomic>
 #include <cmath>
 #include <cstdio>

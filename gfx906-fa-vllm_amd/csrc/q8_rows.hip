@@ -20,6 +20,8 @@ namespace {
 // 8 values of a K row, and of a V chunk 4 values of 4 tokens, which go through
 // LDS to become rows.  Otherwise 16 lanes take a row, 8 values each: one 8-byte
 // K load and 8 dwords of V (each with a byte of the row), four rows at a time.
+// 20001 rows at 8 kv-heads, bf16: 46.7 us with a wave per row and a byte load
+// per V value, 20.5 us in order (126 MB, 6.1 TB/s: HBM).
 struct ReadArgs {
     const uint8_t *kc, *vc;
     const int64_t *slot;
@@ -162,18 +164,19 @@ __global__ __launch_bounds__(256) void read_rows_kernel(ReadArgs a) {
 // K rows are whole pieces of 16 and 8 bytes.  Of a V row every 16-byte chunk
 // holds one byte in four, so V moves by quads of target tokens: a lane loads the
 // target's chunk and those of up to four source rows, merges their bytes and
-// stores the chunk whole (byte stores left the memory with partial lines: 60
-// layers x 32 sequences 34 us, ? us this way).  A path's nodes
-// ascend (a node comes after its parent), so that no row is the target of an
-// earlier one, and a wave moves rows and quads in order, all loads of a step
-// before its stores.  In any other order all rows go through LDS first.
+// stores the chunk whole (with byte stores the lines went out in parts: 60
+// layers x 32 sequences of 26 drafts at 8 kv-heads, 83 rows moved, 34 us, 20.4
+// this way; one layer of 7 sequences 6.2 us, 3.2 of them launch and the rows'
+// places).  A path's nodes ascend (a node comes after its parent), so that no
+// row is the target of an earlier one, and a wave moves rows and quads in order,
+// all loads of a step before its stores.  In any other order all rows go through
+// LDS first.  Bound: runs of 64 to 256 bytes all over the caches, 50 MB of lines
+// in and out for 22 MB of rows (a V row's 128 bytes lie in 512), at 2.5 TB/s.
 constexpr int MAX_DRAFT = 64;
 constexpr int LAYERS = 64;  // layers of one launch, given one by one
-#ifndef GFA_CR_WAVES
-#define GFA_CR_WAVES 8192
-#endif
-constexpr int CR_WAVES = GFA_CR_WAVES;
-constexpr int MAX_QUADS = MAX_DRAFT / 4 + 1;
+// Waves from which a wave takes more than one (layer, kv-head) pair (for the
+// case above 20.4 us; 8192: 21.5, 16384: 23.6).
+constexpr int CR_WAVES = 4096;
 
 struct CompactArgs {
     const int32_t *bt, *seq_lens, *qsl, *accepted, *count;
@@ -223,6 +226,69 @@ __device__ __forceinline__ void piece_store(uint8_t *p, int c, int ts, int td, u
     }
 }
 
+// Piece u of the K rows: row u / 9, piece u % 9.
+struct KPiece {
+    u32x4 x;
+    int r, c, tok;
+    __device__ __forceinline__ void load(const uint8_t *kb, int u, const int64_t *src, const int *toks) {
+        r = u / 9;
+        c = u - 9 * r;
+        tok = toks[r];
+        x = *reinterpret_cast<const u32x4 *>(kb + src[r] + piece_off(c, tok & 15));
+    }
+    __device__ __forceinline__ void store(uint8_t *kb, const int64_t *dst) const {
+        piece_store(kb + dst[r], c, tok & 15, tok >> 8, x);
+    }
+};
+
+// Chunk u % 34 of target quad u / 34 of V: its 16 bytes, and the four rows' that
+// its tokens take (a token without a row takes its own bytes).
+struct VQuad {
+    u32x4 y[4];
+    u32x4 *to;
+    int j, t[4];
+    __device__ __forceinline__ void load(uint8_t *vb, int u, const int64_t *quad, const int (*row)[4],
+                                         const int64_t *src, const int *toks) {
+        const int q = u / CR_QUAD;
+        j = u - CR_QUAD * q;
+        const int at = j < 32 ? (j >> 4) * 1024 + (j & 15) * 16 : SCALE_OFF + (j - 32) * 16;
+        const int per = j < 32 ? 256 : 32;  // bytes of a quad
+        uint8_t *const own = vb + (quad[q] & ~(int64_t)15) + at + per * (int)(quad[q] & 3);
+        to = reinterpret_cast<u32x4 *>(own);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int r = row[q][w];
+            t[w] = r < 0 ? w : toks[r] & 15;
+            y[w] = *reinterpret_cast<const u32x4 *>(r < 0 ? own : vb + src[r] + at + per * (t[w] >> 2));
+        }
+    }
+    __device__ __forceinline__ void store() const {
+        u32x4 x;
+        if (j < 32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t v = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) v |= ((y[w][e] >> (8 * (t[w] & 3))) & 0xFFu) << (8 * w);
+                x[e] = v;
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t h[4];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t d = t[w] & 2 ? y[w][2 * b + 1] : y[w][2 * b];
+                    h[w] = t[w] & 1 ? d >> 16 : d & 0xFFFFu;
+                }
+                x[2 * b] = h[0] | h[1] << 16;
+                x[2 * b + 1] = h[2] | h[3] << 16;
+            }
+        }
+        *to = x;
+    }
+};
+
 __global__ __launch_bounds__(256) void compact_rows_kernel(CompactArgs a) {
     extern __shared__ __attribute__((aligned(16))) u32x4 rows[];  // out of order: [acc_cols][CR_PIECES]
     __shared__ int64_t s_src[MAX_DRAFT], s_dst[MAX_DRAFT];
@@ -270,7 +336,7 @@ __global__ __launch_bounds__(256) void compact_rows_kernel(CompactArgs a) {
         }
     }
     __syncthreads();
-    const int n = s_n;
+    const int n = s_n, nquad = s_nquad;
     if (n == 0) return;
     const int pairs = a.layers * a.Hkv;
     if (s_ascending) {
@@ -279,50 +345,23 @@ __global__ __launch_bounds__(256) void compact_rows_kernel(CompactArgs a) {
             const int64_t head = (int64_t)(p - layer * a.Hkv) * a.chs;
             uint8_t *const kb = (a.list ? a.k[layer] : a.k[0] + layer * a.layer_stride) + head;
             uint8_t *const vb = (a.list ? a.v[layer] : a.v[0] + layer * a.layer_stride) + head;
-            for (int u = lane; u < 9 * n; u += 64) {
-                const int r = u / 9, c = u - 9 * r;
-                const int tok = s_tok[r];
-                const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + s_src[r] + piece_off(c, tok & 15));
-                piece_store(kb + s_dst[r], c, tok & 15, tok >> 8, x);
+            // the first pieces' loads all go out before the first store
+            KPiece k0;
+            VQuad v0, v1;
+            const int nk = 9 * n, nv = CR_QUAD * nquad;
+            if (lane < nk) k0.load(kb, lane, s_src, s_tok);
+            if (lane < nv) v0.load(vb, lane, s_quad, s_row, s_src, s_tok);
+            if (lane + 64 < nv) v1.load(vb, lane + 64, s_quad, s_row, s_src, s_tok);
+            if (lane < nk) k0.store(kb, s_dst);
+            if (lane < nv) v0.store();
+            if (lane + 64 < nv) v1.store();
+            for (int u = lane + 64; u < nk; u += 64) {
+                k0.load(kb, u, s_src, s_tok);
+                k0.store(kb, s_dst);
             }
-            for (int u = lane; u < CR_QUAD * s_nquad; u += 64) {
-                const int q = u / CR_QUAD, j = u - CR_QUAD * q;
-                const int64_t sub = s_quad[q] & ~(int64_t)15;
-                const int at = j < 32 ? (j >> 4) * 1024 + (j & 15) * 16 : SCALE_OFF + (j - 32) * 16;
-                const int per = j < 32 ? 256 : 32;  // bytes of a quad
-                u32x4 *const to = reinterpret_cast<u32x4 *>(vb + sub + at + per * (int)(s_quad[q] & 3));
-                u32x4 x = *to, y[4];
-                int t[4];
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {  // (a token without a row takes its own bytes)
-                    const int r = s_row[q][w];
-                    t[w] = r < 0 ? w : s_tok[r] & 15;
-                    const uint8_t *from = r < 0 ? reinterpret_cast<const uint8_t *>(to)
-                                                : vb + s_src[r] + at + per * (t[w] >> 2);
-                    y[w] = *reinterpret_cast<const u32x4 *>(from);
-                }
-                if (j < 32) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t v = 0;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) v |= ((y[w][e] >> (8 * (t[w] & 3))) & 0xFFu) << (8 * w);
-                        x[e] = v;
-                    }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        uint32_t h[4];
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const uint32_t d = t[w] & 2 ? y[w][2 * b + 1] : y[w][2 * b];
-                            h[w] = t[w] & 1 ? d >> 16 : d & 0xFFFFu;
-                        }
-                        x[2 * b] = h[0] | h[1] << 16;
-                        x[2 * b + 1] = h[2] | h[3] << 16;
-                    }
-                }
-                *to = x;
+            for (int u = lane + 128; u < nv; u += 64) {
+                v0.load(vb, u, s_quad, s_row, s_src, s_tok);
+                v0.store();
             }
         }
         return;
@@ -444,7 +483,7 @@ extern "C" hipError_t gfx906_fa_amd_compact_draft_rows(
         a.layers = nl;
         // (layer, kv-head) pairs a wave takes: more where they alone fill the device
         const int64_t pairs = (int64_t)nl * num_kv_heads;
-        const int64_t each = max((int64_t)1, min((int64_t)8, pairs * num_seqs / CR_WAVES));
+        const int64_t each = max((int64_t)1, min((int64_t)8, (pairs * num_seqs + CR_WAVES - 1) / CR_WAVES));
         const int64_t wgs = min((pairs + 4 * each - 1) / (4 * each), (int64_t)65535);
         compact_rows_kernel<<<dim3(num_seqs, (unsigned)wgs), 256, lds, stream>>>(a);
         const hipError_t e = hipGetLastError();

@@ -177,6 +177,7 @@ constexpr int LAYERS = 64;  // layers of one launch, given one by one
 // Waves from which a wave takes more than one (layer, kv-head) pair (for the
 // case above 20.4 us; 8192: 21.5, 16384: 23.6).
 constexpr int CR_WAVES = 4096;
+constexpr int MAX_QUADS = MAX_DRAFT / 4 + 1;
 
 struct CompactArgs {
     const int32_t *bt, *seq_lens, *qsl, *accepted, *count;

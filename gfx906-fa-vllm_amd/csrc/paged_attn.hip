@@ -3889,7 +3889,15 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
             else
                 attn_combine_kernel<1, ODT><<<dim3(num_seqs, num_kv_heads, crow), 256, 0, stream>>>(pd);
         } else if (c.nrg == 3) {
-            attn_decode_kernel<3, QDT, ODT, false, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
+            // Scored tiles keep K^'s ints and a cap's or a tree's operands in
+            // registers besides: with three row groups they spill, and 48 rows
+            // are faster as two chunks of 32 (fp16, from graphs: a tree of 8
+            // nodes on 8 x 32768 keys at 6/1 54.0 -> 42.5 us, on 8 x 8192 at
+            // 48/8 79.9 -> 64.3).  The slots stay those of 48 rows.
+            if constexpr (SC == SC_NONE)
+                attn_decode_kernel<3, QDT, ODT, false, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
+            else
+                attn_decode_kernel<2, QDT, ODT, true, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);
             if (merge) attn_combine_kernel<3, ODT><<<dim3(num_seqs, num_kv_heads, crow), 256, 0, stream>>>(pd);
         } else {
             if (c.rows_hi > 32) attn_decode_kernel<2, QDT, ODT, true, SC><<<c.nwg, 64 * DEC_NW, 0, stream>>>(pd);

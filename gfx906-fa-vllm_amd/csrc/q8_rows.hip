@@ -451,6 +451,14 @@ extern "C" hipError_t gfx906_fa_amd_compact_draft_rows(
         fprintf(stderr, "[gfx906_fa_amd] compact_draft_rows: caches must be 16-byte aligned\n");
         return hipErrorInvalidValue;
     }
+    // one cache as two layers would be compacted twice, by waves that race
+    bool twice = !list && num_layers > 1 && layer_stride == 0;
+    for (int i = 0; list && i < num_layers; ++i)
+        for (int j = 0; j < i; ++j) twice = twice || k_layers[i] == k_layers[j] || v_layers[i] == v_layers[j];
+    if (twice) {
+        fprintf(stderr, "[gfx906_fa_amd] compact_draft_rows: two layers share a cache\n");
+        return hipErrorInvalidValue;
+    }
     if (num_seqs == 0 || num_layers == 0 || accepted_cols == 0) return hipSuccess;
     if ((int64_t)num_layers * num_kv_heads > (1 << 24)) {
         fprintf(stderr, "[gfx906_fa_amd] compact_draft_rows: too many layers\n");

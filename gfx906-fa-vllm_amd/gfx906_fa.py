@@ -766,7 +766,10 @@ def tree_masks(parents) -> torch.Tensor:
     node: one sequence's list, or a list of them, one per sequence.  A node's
     parent comes before it; a root's is -1.  Bit i of a node's mask: node i is
     it or one of its ancestors."""
-    trees = [list(parents)] if not len(parents) or isinstance(parents[0], int) else [list(t) for t in parents]
+    if hasattr(parents, "tolist"):  # an array or a tensor
+        parents = parents.tolist()
+    trees = [t.tolist() if hasattr(t, "tolist") else list(t)
+             for t in (parents if len(parents) and hasattr(parents[0], "__len__") else [parents])]
     out = []
     for tree in trees:
         _check(len(tree) <= MAX_TREE_NODES, f"a tree has at most {MAX_TREE_NODES} nodes, got {len(tree)}")
@@ -920,7 +923,8 @@ def compact_draft_rows(kv_caches, block_table: torch.Tensor, seq_lens: torch.Ten
 
     ``kv_caches``: one stacked tensor, uint8 [layers, NB, 2, Hkv, bs/16*2176],
     or a sequence of (key_cache, value_cache) planes, one pair per layer, of
-    one shape and one set of strides.  Sequences must not share draft pages."""
+    one shape and one set of strides; a cache that several layers share counts
+    once.  Sequences must not share draft pages."""
     kp = vp = None
     if isinstance(kv_caches, torch.Tensor):
         shape = kv_caches.shape
@@ -948,7 +952,10 @@ def compact_draft_rows(kv_caches, block_table: torch.Tensor, seq_lens: torch.Ten
             if not (k.shape == v.shape == shape and k.stride() == v.stride() == strides
                     and k.dtype == v.dtype == torch.uint8 and k.get_device() == v.get_device() == at):
                 raise RuntimeError("every layer's planes must be uint8 of one shape, set of strides and device")
-        kp, vp = ((ctypes.c_void_p * layers)(*[p[i].data_ptr() for p in pairs]) for i in range(2))
+        # layers that share a cache (KV sharing) are one: its rows move once
+        ptrs = dict.fromkeys((k.data_ptr(), v.data_ptr()) for k, v in pairs)
+        layers = len(ptrs)
+        kp, vp = ((ctypes.c_void_p * layers)(*p) for p in zip(*ptrs))
     if at < 0:
         raise RuntimeError("kv_caches must be CUDA/HIP")
     if not (block_table.get_device() == seq_lens.get_device() == query_start_loc.get_device() == accepted.get_device()

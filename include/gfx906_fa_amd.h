@@ -521,7 +521,8 @@ hipError_t gfx906_fa_amd_read_rows(
  *     outside the block table and pages outside [0, num_blocks) are skipped.
  *     The layers' planes: k_layers / v_layers (host arrays of num_layers device
  *     pointers), or, with those NULL, k_cache / v_cache + layer * layer_stride
- *     bytes.  All layers share the page strides (bytes) and the block table. */
+ *     bytes.  All layers share the page strides (bytes) and the block table, and
+ *     no two a plane (refused). */
 hipError_t gfx906_fa_amd_compact_draft_rows(
     uint8_t *const *k_layers, uint8_t *const *v_layers, uint8_t *k_cache, uint8_t *v_cache, int64_t layer_stride,
     int num_layers, int64_t cache_block_stride, int64_t cache_head_stride, int64_t num_blocks, const int32_t *block_table,

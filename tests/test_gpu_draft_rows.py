@@ -71,6 +71,28 @@ def test_compact(bs, layers, Hkv, how):
     assert np.array_equal(stack.cpu().numpy(), want)
 
 
+def test_layers_that_share_a_cache_move_once():
+    need_gpu()
+    announce("shared layers")
+    rng = np.random.default_rng(8)
+    ctx, nq, layers = [13, 40], [12, 30], [0, 1, 0, 2, 1, 0]
+    bt, nb = _tables(rng, [c + n for c, n in zip(ctx, nq)], 16)
+    acc = np.full((2, 8), -1, np.int32)
+    acc[0, :4], acc[1] = [0, 2, 3, 9], np.arange(8)[::-1]  # targets that are sources of other rows
+    count = np.array([4, 8], np.int32)
+    stack = torch.randint(0, 256, (3, nb, 2, 2, 2176), dtype=torch.uint8, device=DEV)
+    want = stack.cpu().numpy().copy()
+    for layer in want:
+        _compact_ref(layer, bt, ctx, nq, acc, count)
+    t = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV)  # noqa: E731
+    args = (t(bt), t([c + n for c, n in zip(ctx, nq)]), t(np.concatenate([[0], np.cumsum(nq)])), t(acc), t(count))
+    with pytest.raises(RuntimeError):
+        gfx906_fa.compact_draft_rows(stack[:1].expand(2, -1, -1, -1, -1), *args)
+    gfx906_fa.compact_draft_rows([(stack[i, :, 0], stack[i, :, 1]) for i in layers], *args)
+    torch.cuda.synchronize()
+    assert np.array_equal(stack.cpu().numpy(), want)
+
+
 def test_compact_skips_what_it_cannot_reach():
     """Missing pages, short tables and lengths below the drafts move nothing."""
     need_gpu()

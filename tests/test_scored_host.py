@@ -21,6 +21,9 @@ def test_tree_masks():
     for bad in ([0], [-1, 1], [-2], [-1] * 65):
         with pytest.raises(RuntimeError):
             gfx906_fa.tree_masks(bad)
+    tree = torch.tensor([-1, 0, 0, 2])
+    for same in (tree, tree.numpy(), list(tree.numpy()), [tree], [tree.numpy()], tree[None]):
+        assert gfx906_fa.tree_masks(same).tolist() == [1, 3, 5, 13]
 
 
 def test_oracle_visibility():
@@ -80,6 +83,17 @@ def test_row_entries_refusals():
         bad = list(comp)
         bad[at] = value
         assert L.gfx906_fa_amd_compact_draft_rows(*bad) == 1, (at, value)
+
+
+def test_compact_refuses_one_cache_as_two_layers():
+    L = gfx906_fa.lib()
+    p = ctypes.c_void_p(256)
+    rest = [4352, 2176, 4, p, 2, 2, p, p, p, 4, 4, p, 1, 1, 128, 16, None]
+    assert L.gfx906_fa_amd_compact_draft_rows(None, None, p, p, 0, 2, *rest) == 1
+    planes = lambda *a: (ctypes.c_void_p * len(a))(*a)  # noqa: E731
+    far = [1 << 20 | i << 8 for i in range(70)]
+    for k, v in (([256, 256], [512, 1024]), ([256, 512], [1024, 1024]), (far[:69] + far[:1], [x + 65536 for x in far])):
+        assert L.gfx906_fa_amd_compact_draft_rows(planes(*k), planes(*v), None, None, 0, len(k), *rest) == 1
 
 
 def test_host_tensors_are_refused():

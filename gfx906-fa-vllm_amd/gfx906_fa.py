@@ -632,8 +632,11 @@ def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_lo
     if at < 0:
         _cuda(query, "query")
     if not (key_cache.get_device() == value_cache.get_device() == block_table.get_device() == seq_lens.get_device()
-            == query_start_loc.get_device() == at) or any(
-                t is not None and t.get_device() != at for t in (alibi_slopes, tree_mask, out, workspace, q_abs_offset)):
+            == query_start_loc.get_device() == at
+            and (alibi_slopes is None or alibi_slopes.get_device() == at)
+            and (tree_mask is None or tree_mask.get_device() == at) and (out is None or out.get_device() == at)
+            and (workspace is None or workspace.get_device() == at)
+            and (q_abs_offset is None or q_abs_offset.get_device() == at)):
         _all_on(at, (key_cache, value_cache, block_table, seq_lens, query_start_loc, alibi_slopes, tree_mask, out,
                      workspace, q_abs_offset),
                 "key_cache value_cache block_table seq_lens query_start_loc alibi_slopes tree_mask out workspace "
@@ -688,7 +691,7 @@ def _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_lo
         _check(q_abs_offset.dtype == torch.int32 and q_abs_offset.is_contiguous()
                and q_abs_offset.shape[0] >= B, "q_abs_offset must be int32 [B]")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=out_dtype or dt, device=dev)
+        out = torch.empty(T, Hq, D, dtype=out_dtype or dt, device=dev)
         odt, ots, ohs = _DT[out_dtype or dt], Hq * D, D
     else:
         oshape, (ots, ohs, os) = out.shape, out.stride() if out.dim() == 3 else (0, 0, 0)
@@ -867,8 +870,8 @@ def read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_
     at = slot_mapping.get_device()
     if at < 0:
         _cuda(slot_mapping, "slot_mapping")
-    if not (key_cache.get_device() == value_cache.get_device() == at) or any(
-            t is not None and t.get_device() != at for t in (k_out, v_out)):
+    if not (key_cache.get_device() == value_cache.get_device() == at and (k_out is None or k_out.get_device() == at)
+            and (v_out is None or v_out.get_device() == at)):
         _all_on(at, (key_cache, value_cache, k_out, v_out), "key_cache value_cache k_out v_out")
     if _get_device() != at:
         with torch.cuda.device(at):
@@ -882,8 +885,8 @@ def read_cache_q8_kv(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_
     T = slot_mapping.shape[0]
     dev = slot_mapping.device
     if k_out is None and v_out is None:
-        k = torch.empty((T, Hkv, 128), dtype=dtype, device=dev)
-        v = torch.empty((T, Hkv, 128), dtype=dtype, device=dev)
+        k = torch.empty(T, Hkv, 128, dtype=dtype, device=dev)
+        v = torch.empty_like(k)
         kts = vts = Hkv * 128
         khs = vhs = 128
     else:

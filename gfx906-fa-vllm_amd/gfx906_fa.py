@@ -741,8 +741,8 @@ def scored_paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_c
     One of the two, or neither (plain attention).  query fp16 or bf16 [T, Hq,
     128]; out of its dtype or fp32.  Lengths, workspace and errors as
     ``paged_attention``: ``max_query_len`` / ``max_seq_len`` must bound the
-    device values.  A row that sees no key is 0; what the cache holds past a
-    sequence's keys does not matter, NaN and Inf included."""
+    device values.  A row that sees no key is 0; with a cap or slopes, what the
+    cache holds past a sequence's keys does not matter, NaN and Inf included."""
     return _scored(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, max_query_len, max_seq_len,
                    scale, soft_cap, alibi_slopes, None, out, workspace, q_abs_offset, causal, out_dtype)
 
@@ -794,8 +794,8 @@ def qk_norm_rope_and_cache_q8_kv(positions: torch.Tensor, query: torch.Tensor, k
     x * rsqrt(mean(x^2) + eps) * weight (``query_weight`` / ``key_weight`` [128],
     the model dtype), then its first rot_dim values are rotated, in place, in
     fp32 and rounded once; the stored key and the value go to the cache as Q8_0
-    at slot_mapping (slots outside the cache, < 0 too, are skipped).  One launch.  Rows at positions outside
-    [0, max_position) are normed and not rotated."""
+    at slot_mapping (slots outside the cache, < 0 too, are skipped).  One launch.
+    Rows at positions outside [0, max_position) are normed and not rotated."""
     at = query.get_device()
     if at < 0:
         _cuda(query, "query")

@@ -470,9 +470,9 @@ hipError_t gfx906_fa_amd_paged_attention_padded(
  *                     64.
  *     soft_cap and tree_mask go together; alibi_slopes alone.  Without any of
  *     them the call is (5).  query fp16 or bf16, out of its type or fp32.
- *     Workspace and plan as (5).  A row that sees no key is 0.  K and V of
- *     keys that no row sees, or that some row does not see, may hold anything;
- *     a V block a row sees has to have a finite scale. */
+ *     Workspace and plan as (5).  A row that sees no key is 0.  With one of
+ *     them, K and V of keys that no row sees, or that some row does not see,
+ *     may hold anything; a V block a row sees has to have a finite scale. */
 hipError_t gfx906_fa_amd_scored_paged_attention(
     const void *q, int q_dtype, int64_t q_token_stride, int64_t q_head_stride,
     const uint8_t *k_cache, const uint8_t *v_cache, int64_t cache_block_stride,

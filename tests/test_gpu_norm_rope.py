@@ -91,6 +91,15 @@ def test_heads_and_lengths(T, Hq, Hkv, bs):
     _run("bf16", T, Hq, Hkv, 128, True, "model", bs=bs, seed=T)
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,bs,rot,neox", [(1100, 48, 8, 16, 128, True), (1237, 48, 8, 32, 64, False),
+                                                   (2050, 16, 16, 64, 96, True)])
+def test_many_tokens(T, Hq, Hkv, bs, rot, neox):
+    """Past 2048 waves: 16 rows a wave, nontemporal, a last run of workgroups that is cut."""
+    need_gpu()
+    announce(f"norm rope T={T} {Hq}/{Hkv} bs={bs}")
+    _run("f16", T, Hq, Hkv, rot, neox, "f32", bs=bs, seed=T)
+
+
 @pytest.mark.parametrize("spread", [1e-4, 300.0])
 @pytest.mark.parametrize("eps", [0.0, 1e-5, 1.0])
 def test_magnitudes(spread, eps):

@@ -1289,9 +1289,9 @@ __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void at
         WaveAcc<NRG> acc;
         acc_init(acc);
         // verify tiles and the scored forms: sub-pages staged through this
-        // wave's sm_o slice.  (One row group of the scored forms with two
-        // sub-pages in registers instead, 64 of them: 20 spilled, 32 x 2K-16K
-        // capped 100 us.)
+        // wave's sm_o slice.  (One row group of the scored forms, 32 x 2K-16K
+        // capped: 80 us, 5.8 TB/s; with two sub-pages in 64 registers instead 20
+        // spill, 100 us.)
         if constexpr (RING) {
             static_assert(sizeof(sm_o[0]) >= DEC_RING * DEC_RING_SLOT, "ring fits the wave's slice");
             stream_range_lds<NRG, DEC_RING, SC>(acc, p, s, h, 16 * a, min(16 * b, si.kv_lim), qf, lim, sr, lane, i16,
@@ -1739,9 +1739,6 @@ __device__ __forceinline__ void pf_dequant_v(const PfRaw &r, uint8_t *vst, int s
 // them there), whose V rows are the caller's own.  An instance of its own: the
 // clearing of unseen V in the paged instance's copy loop cost the 32K prompt
 // 1 % (11.07 -> 11.2 ms), though it never ran there.
-#ifndef GFA_PF_QLDS
-#define GFA_PF_QLDS 4
-#endif
 template <int QDT, int ODT, bool VF16, bool MASK, int KS = 1, bool FLAT = false, int SC = SC_NONE>
 __global__ __launch_bounds__(64 * PF_WAVES)
 __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p) {
@@ -1753,10 +1750,12 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
     // into the stages 1 and 2, free until the first tile has been written)
     constexpr int STAGES = NSTAGE * (PF_KBYTES + PF_VBYTES);
     // Q fragments that stay in LDS between the tiles (KS = 1: a lane's own 16
-    // bytes each; KS = 2: where the Q rows are).  The capped scores' temporaries do not fit beside all eight in
-    // registers: the compiler spilled two of them, and the QK waited for them
-    // to come back from memory in every tile.
-    constexpr int QLDS = SC == SC_CAP ? GFA_PF_QLDS : 0;
+    // bytes each; KS = 2: where the Q rows are).  The capped scores' temporaries
+    // do not fit beside all eight in registers: the compiler spilled two of them,
+    // and the QK waited for them to come back from memory in every tile (a prompt
+    // of 8192 at 48/8: 1145 -> 990 us).  Its VALU (66 % of the cycles) and MFMA (41
+    // %) about add up: 0.85 PFLOP/s.
+    constexpr int QLDS = SC == SC_CAP ? 4 : 0;
     __shared__ __attribute__((aligned(16))) uint8_t lds[STAGES + PF_CWAVES * (KS == 2 ? PF_QBYTES : QLDS * 1024)];
     uint8_t *const ldsk = lds;
     uint8_t *const ldsv = lds + NSTAGE * PF_KBYTES;

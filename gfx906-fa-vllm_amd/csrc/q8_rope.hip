@@ -395,21 +395,23 @@ __device__ __forceinline__ void load_cs_f32(const void *row, int col, float (&v)
     for (int e = 0; e < N; e += 2) load2_as_f32<CSDT>(row, col + e, v[e], v[e + 1]);
 }
 
-// Rows per wave: 4 x 4, or 4 x 2 below NORM_FEW_WAVES waves of 32 rows, so that
+// Rows per wave: 4 x 4, or 4 x 2 below NORM_FEW_WAVES waves of 16 rows, so that
 // more waves share few tokens (64 tokens at 48/8: 5.9 us with 32 rows a wave,
-// 5.0 with 8; 8192 tokens: 68.4 us with 32, 66.2 with 16, 73.2 with 8).
+// 5.0 with 8; 8192 tokens: 68.4 us with 32, 66.2 with 16, 73.2 with 8).  16
+// against 8 rows, bf16, buffers out of cache: 1024 waves (16/16, 512 tokens) 7.8
+// and 6.8 us; 2048 (48/8, 512; 16/16, 1024) 6.6 and 7.8, 9.8 and 9.7; 4096 (48/8,
+// 1024) 9.3 and 11.8.
 constexpr int NORM_ITERS = 4, NORM_FEW_ITERS = 2;
-#ifndef GFA_NORM_FEW_WAVES
-#define GFA_NORM_FEW_WAVES 2048
-#endif
-constexpr int NORM_FEW_WAVES = GFA_NORM_FEW_WAVES;
+constexpr int NORM_FEW_WAVES = 2048;
 
 template <int DT, int CSDT, bool NEOX, int ITERS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q8_norm_rope_cache_write_kernel(NormArgs n) {
     const RopeArgs &a = n.r;
-    // Many tokens stream through once, more than the caches hold for the
-    // attention to find: nontemporal both ways (8192 tokens at 48/8, bf16, 66.5
-    // -> 59.7 us, 4.55 TB/s; loads alone 63.7, stores alone 64.9).
+    // Many tokens stream through once: nontemporal both ways (8192 tokens at
+    // 48/8, bf16, 66.5 -> 59.7 us, 4.55 TB/s; loads alone 63.7, stores alone
+    // 64.9).  Between the store of the projection and a reader of the query the
+    // three take 132.2 -> 131.3 us for 8192 tokens, 68.0 -> 68.2 for 4096, 281 ->
+    // 257 for 16384.
     constexpr bool NT = ITERS > 2;
     auto load = [](const uint16_t *p) __attribute__((always_inline)) {
         const u32x4_t *v = reinterpret_cast<const u32x4_t *>(p);
@@ -530,7 +532,7 @@ template <int DT, int CSDT>
 hipError_t launch_norm_rope(const NormArgs &a, bool neox, hipStream_t stream) {
     NormArgs n = a;
     const int rows = a.r.Hq + a.r.Hkv;
-    const bool few = a.r.num_tokens * ((rows + 31) / 32) < NORM_FEW_WAVES;
+    const bool few = a.r.num_tokens * ((rows + 15) / 16) < NORM_FEW_WAVES;
     const int per = 4 * (few ? NORM_FEW_ITERS : NORM_ITERS);
     n.r.nchunk = (rows + per - 1) / per;
     const int64_t blocks = (a.r.num_tokens * n.r.nchunk + 3) / 4;

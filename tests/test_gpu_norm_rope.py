@@ -94,7 +94,7 @@ def test_heads_and_lengths(T, Hq, Hkv, bs):
 @pytest.mark.parametrize("T,Hq,Hkv,bs,rot,neox", [(1100, 48, 8, 16, 128, True), (1237, 48, 8, 32, 64, False),
                                                    (2050, 16, 16, 64, 96, True)])
 def test_many_tokens(T, Hq, Hkv, bs, rot, neox):
-    """Past 2048 waves: 16 rows a wave, nontemporal, a last run of workgroups that is cut."""
+    """From 2048 waves of 16 rows on: 16 rows a wave, nontemporal, a last run of workgroups that is cut."""
     need_gpu()
     announce(f"norm rope T={T} {Hq}/{Hkv} bs={bs}")
     _run("f16", T, Hq, Hkv, rot, neox, "f32", bs=bs, seed=T)

@@ -3597,12 +3597,14 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 // (a kmul up to 2 would overflow keys above 65504 / kmul, 32.8K at worst).
 // Capped scores carry 2 log2 e * scale / cap instead, far below 1 for the usual
 // caps: below 2^-8 K^ takes the rest (its ints times a scale near 1 / 127 of
-// the keys keep their bits down to 2^-7 of that).
+// the keys keep their bits down to 2^-7 of that).  Caps far below the scale give
+// up to 92: past 2^3 K^ takes the rest, so that queries up to 8K and keys up to
+// 5.6K stay finite in fp16.
 void set_prefill_scale(AttnParams &p, bool capped) {
     int e = 0;
     (void)frexpf(p.scale_log2e, &e);  // c = m * 2^e, m in [0.5, 1)
     e = max(-60, min(60, -e));
-    if (capped) e = min(e, 8);
+    if (capped) e = max(-3, min(e, 8));
     p.pf_qmul = ldexpf(1.0f, -e);
     p.pf_kmul = ldexpf(p.scale_log2e, e);
 }

@@ -91,6 +91,17 @@ def test_cap_range(name, cap):
     check(out, *scored_oracle(b, cap=cap))
 
 
+@pytest.mark.parametrize("spread", [1500.0, 0.01])
+@pytest.mark.parametrize("name", ["prompts", "rows96", "decode"])
+def test_small_cap_of_large_scores(name, spread):
+    """The cap far below the scale, queries far from 1 (the largest about 6000)."""
+    need_gpu()
+    announce(f"small cap {name} {spread}")
+    b = _batch(name, "f16", spread=spread)
+    out = _call(b, soft_cap=0.003, out_dtype=torch.float32)
+    check(out, *scored_oracle(b, cap=0.003))
+
+
 @pytest.mark.parametrize("name", ["decode", "verify30", "prompts"])
 def test_slopes_of_any_sign_and_size(name):
     need_gpu()

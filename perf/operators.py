@@ -18,7 +18,6 @@ elementary torch operations in 32 bits.  Lengths are ragged and drawn from the
 case's own ``lens`` number, so that a case always has the same sizes; block
 tables are random permutations of the pool.
 """
-import functools
 import math
 import os
 import random
@@ -306,8 +305,7 @@ def _prepare_compact(case, seed):
 
 
 # --- one pass --------------------------------------------------------------------------------------
-@functools.lru_cache(None)
-def _framework():  # a program imports it once
+def _framework():
     at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gfx906-fa-vllm_amd")
     if at not in sys.path:
         sys.path.insert(1, at)

@@ -1682,7 +1682,8 @@ __device__ __forceinline__ half8_t scale8_f32(half8_t v, float s) {
 // of the tile): K^ rows into kst, V^T columns into vst.  TAIL (the last tile
 // of the range, the only one that can hold keys past kv_end): bytes of tokens
 // past the valid range are dequantized as they are - their scores are masked
-// to -inf (P = 0) - and the V scales are made finite so that 0 * V^ stays 0.
+// to -inf (P = 0) - and V^ itself is made finite so that 0 * V^ stays 0 (not
+// its scale: a finite one times an int can pass 65504 as well).
 // K^ carries the part kmul = c * 2^e of the softmax scale c = scale * log2 e
 // (Q carries the exact power of two 2^-e): K^ = fp16(q * (d * kmul)), the
 // product formed in fp32 and rounded once.  Pre-scaling Q by c in fp16 would
@@ -1721,16 +1722,16 @@ __device__ __forceinline__ void pf_dequant_v(const PfRaw &r, uint8_t *vst, int s
 #pragma unroll
     for (int mm = 0; mm < 4; ++mm) {
         const int b = mm >> 1;  // block 2hf + b: scale dwords 2b (tokens 0,1), 2b+1 (2,3)
-        half2_t s01 = __builtin_bit_cast(half2_t, vsw[2 * b]);
-        half2_t s23 = __builtin_bit_cast(half2_t, vsw[2 * b + 1]);
-        if (TAIL) {
-            s01 = finite2(s01);
-            s23 = finite2(s23);
-        }
+        const half2_t s01 = __builtin_bit_cast(half2_t, vsw[2 * b]);
+        const half2_t s23 = __builtin_bit_cast(half2_t, vsw[2 * b + 1]);
         half2_t lo, hi;
         i8x4_to_f16x4(vq[mm], lo, hi);
         lo *= s01;
         hi *= s23;
+        if (TAIL) {
+            lo = finite2(lo);
+            hi = finite2(hi);
+        }
         *reinterpret_cast<half4_t *>(vcol + 16 * mm * PF_VPITCH) = half4_t{lo[0], lo[1], hi[0], hi[1]};
     }
 }
@@ -1949,8 +1950,8 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
         };
         auto dequant_v = [&](const PfRawT &rw, int t, auto tail) __attribute__((always_inline)) {
             uint8_t *vst = ldsv + (t % NSTAGE) * PF_VBYTES;
-            // (a scored form may hide keys of the tiles before the last: its V
-            // scales are made finite in every tile)
+            // (a scored form may hide keys of the tiles before the last: its V^
+            // is made finite in every tile)
             constexpr bool T = decltype(tail)::value || SC != SC_NONE;
             pf_dequant_v<T, VF16>(rw.h[0], vst, wsp, lane, 0);
             pf_dequant_v<T, VF16>(rw.h[1], vst, wsp, lane, 1);

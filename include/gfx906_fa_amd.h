@@ -185,6 +185,10 @@ hipError_t gfx906_fa_amd_rope_cache_write_kv(
  *       k <= q_abs_offset[s] + j   (q_abs_offset may be NULL: then
  *                                   q_abs_offset[s] = seq_lens[s] - n_q[s]).
  *     q-head hq reads kv-head hq / (Hq/Hkv).  A row with no visible key is 0.
+ *     Bytes behind a sequence's last key may hold anything, but decode-shaped
+ *     sequences need finite V scales there (a zeroed or recycled page's are).
+ *     Prefill-shaped ones hold V in fp16: values a row sees have to lie within
+ *     +-65504.
  *     Numerics: dequantize-then-fp32 softmax (scores, max, sum and output
  *     accumulated in fp32; K int8 values enter the MFMA exactly and their
  *     scales are applied to the fp32 products; V scales are folded into P).
@@ -472,7 +476,9 @@ hipError_t gfx906_fa_amd_paged_attention_padded(
  *     them the call is (5).  query fp16 or bf16, out of its type or fp32.
  *     Workspace and plan as (5).  A row that sees no key is 0.  With one of
  *     them, K and V of keys that no row sees, or that some row does not see,
- *     may hold anything; a V block a row sees has to have a finite scale. */
+ *     may hold anything; a V block a row sees has to have a finite scale, and
+ *     values within +-65504 where the row is of a prefill-shaped sequence
+ *     (larger ones count as +-65504 there). */
 hipError_t gfx906_fa_amd_scored_paged_attention(
     const void *q, int q_dtype, int64_t q_token_stride, int64_t q_head_stride,
     const uint8_t *k_cache, const uint8_t *v_cache, int64_t cache_block_stride,

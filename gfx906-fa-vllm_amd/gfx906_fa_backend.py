@@ -28,7 +28,7 @@ What differs, by design:
 from __future__ import annotations
 
 import os
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import ClassVar
 
 import torch
@@ -74,8 +74,60 @@ class Gfx906FAMetadata:
     use_cascade: bool = False
     common_prefix_len: int = 0
     # int64 [num_tokens]: the step verifies a tree of drafts per sequence
-    # (gfx906_fa.tree_masks); None: causal rows
+    # (gfx906_fa.tree_masks; -1: a causal row); None: causal rows
     tree_mask: torch.Tensor | None = None
+    # the builder's: what tree_mask is told to
+    graph_masks: _GraphMasks | None = field(default=None, repr=False, compare=False)
+
+    def __post_init__(self) -> None:
+        if self.tree_mask is not None:  # (given to the constructor)
+            self.tree_mask = self.tree_mask
+
+    def __setattr__(self, name: str, value) -> None:
+        graphs = self.__dict__.get("graph_masks")
+        if name == "tree_mask" and graphs is not None:
+            graphs.set(self, value)
+        super().__setattr__(name, value)
+
+
+class _GraphMasks:
+    """The tree masks that the graphs captured from a builder's metadata read: a
+    buffer of its own where trees are enabled (GFX906_FA_TREES=1), -1 (causal
+    rows) wherever the step has no masks.  Without one, a mask for a step that
+    such a graph would replay is refused: the graph is a causal step's."""
+
+    def __init__(self, rows: int | None, device: torch.device) -> None:
+        self.buffer = None if rows is None else torch.full((rows,), -1, dtype=torch.int64, device=device)
+        self.captured: set[int] = set()  # query lengths of the captured batches
+        self._masks = False
+
+    def __deepcopy__(self, memo):
+        return self  # (a copied metadata is still a step of this builder's)
+
+    def causal(self) -> None:
+        if self._masks:
+            self.buffer.fill_(-1)
+            self._masks = False
+
+    def set(self, md: Gfx906FAMetadata, masks: torch.Tensor | None) -> None:
+        if self.buffer is None:
+            if masks is not None and md.max_query_len in self.captured:
+                raise RuntimeError(
+                    f"GFX906_FA: steps of {md.max_query_len} tokens a sequence were captured into graphs as causal "
+                    "steps; set GFX906_FA_TREES=1 for graphs that read tree masks")
+            return
+        if masks is not None and masks.data_ptr() == self.buffer.data_ptr():
+            return  # (the captured steps' own)
+        self.causal()
+        if masks is None:
+            return
+        n = md.num_actual_tokens
+        if masks.dtype != torch.int64 or masks.dim() != 1 or not n <= masks.shape[0]:
+            raise RuntimeError("GFX906_FA: tree_mask must be int64 [num_tokens]")
+        if n > self.buffer.shape[0]:
+            raise RuntimeError(f"GFX906_FA: {n} tokens exceed max_num_batched_tokens ({self.buffer.shape[0]})")
+        self.buffer[:n].copy_(masks[:n])
+        self._masks = True
 
 
 def workspace_upper_bound(max_num_seqs: int, max_num_tokens: int, heads, max_seq_len: int = -1,
@@ -149,17 +201,35 @@ class Gfx906FAMetadataBuilder(AttentionMetadataBuilder[Gfx906FAMetadata]):
                 pass
         if limits is not None and heads and torch.device(device).type == "cuda":
             Gfx906FAImpl.reserve_workspace(Gfx906FAImpl.bound_bytes(heads, limits), torch.device(device))
+        rows = None
+        if os.environ.get("GFX906_FA_TREES", "0") == "1":
+            if limits is None:
+                raise ValueError("GFX906_FA_TREES=1 needs the scheduler's max_num_seqs and max_num_batched_tokens")
+            rows = limits[1]
+        self._graph_masks = _GraphMasks(rows, device)
 
     def build_for_cudagraph_capture(self, common_attn_metadata: CommonAttentionMetadata
                                     ) -> Gfx906FAMetadata:
         # a graph captured from here keeps the workspace's raw address: from
         # now on a replaced workspace must stay allocated
         Gfx906FAImpl._captured = True
-        return self.build(0, common_attn_metadata)
+        md = self.build(0, common_attn_metadata)
+        masks = self._graph_masks
+        masks.captured.add(md.max_query_len)
+        if masks.buffer is not None and md.max_query_len <= gfx906_fa.MAX_TREE_NODES:
+            # the graph's launches read the masks of the step that replays it
+            if md.num_actual_tokens > masks.buffer.shape[0]:
+                raise RuntimeError(f"GFX906_FA: {md.num_actual_tokens} tokens exceed max_num_batched_tokens "
+                                   f"({masks.buffer.shape[0]})")
+            md.__dict__["tree_mask"] = masks.buffer[:md.num_actual_tokens]
+        return md
 
     def build(self, common_prefix_len: int, common_attn_metadata: CommonAttentionMetadata,
               fast_build: bool = False) -> Gfx906FAMetadata:
-        return Gfx906FAMetadata(
+        """A step's metadata.  With GFX906_FA_TREES=1 its ``tree_mask``, set
+        before the step runs or replays, also reaches the graphs captured from
+        this builder; they show causal rows again from the next build() on."""
+        md = Gfx906FAMetadata(
             num_actual_tokens=common_attn_metadata.num_actual_tokens,
             max_query_len=common_attn_metadata.max_query_len,
             max_seq_len=common_attn_metadata.max_seq_len,
@@ -169,7 +239,10 @@ class Gfx906FAMetadataBuilder(AttentionMetadataBuilder[Gfx906FAMetadata]):
             slot_mapping=common_attn_metadata.slot_mapping,
             use_cascade=(common_prefix_len > 0),
             common_prefix_len=common_prefix_len,
+            graph_masks=self._graph_masks,
         )
+        self._graph_masks.causal()
+        return md
 
 
 # -----------------------------------------------------------------------------

@@ -84,6 +84,10 @@ class Gfx906FAMetadata:
             self.tree_mask = self.tree_mask
 
     def __setattr__(self, name: str, value) -> None:
+        if name == "tree_mask" and value is not None and self.max_query_len > gfx906_fa.MAX_TREE_NODES:
+            # (a mask has 64 bits: a longer chunk's rows cannot be said in it)
+            raise RuntimeError(f"GFX906_FA: a tree step has at most {gfx906_fa.MAX_TREE_NODES} query tokens a sequence "
+                               f"(max_query_len {self.max_query_len}); longer prompt chunks go into a step of their own")
         graphs = self.__dict__.get("graph_masks")
         if name == "tree_mask" and graphs is not None:
             graphs.set(self, value)

@@ -57,3 +57,22 @@ def test_captured_step_replays_the_steps_masks(monkeypatch, heads, n, cap):
         check(eager.view(2 * n, b.Hq, 128), ref, bound)
         if not causal:
             assert torch.equal(out, eager)
+
+
+def test_causal_sequences_beside_trees():
+    """A tree step with a decode, a linear draft and prompt chunks of up to 64
+    tokens, whose rows have the mask -1."""
+    need_gpu()
+    announce("tree step with causal sequences")
+    from gfx906_fa_backend import Gfx906FAImpl
+    lens, nq = [300, 64, 420, 64, 90], [7, 1, 64, 64, 5]
+    impl, b, kv, md = _layer(Gfx906FAImpl, "auto", lens, nq, 12, 2)
+    masks = torch.full((sum(nq),), -1, dtype=torch.int64)
+    masks[:7] = gfx906_fa.tree_masks(random_tree(np.random.default_rng(4), 7))
+    md.tree_mask = masks.to(DEV)
+    out = torch.empty((b.num_tokens, b.Hq * 128), dtype=torch.bfloat16, device=DEV)
+    impl.forward(None, b.query, None, None, kv, md, output=out)
+    out = out.view(b.num_tokens, b.Hq, 128)
+    check(out, *scored_oracle(b, masks=masks.numpy(), out_eps=eps_of(torch.bfloat16)))
+    ref, bound = scored_oracle(b, out_eps=eps_of(torch.bfloat16))  # causal rows
+    check(out[7:], ref[7:], bound[7:])

@@ -106,3 +106,20 @@ def test_metadata_made_by_hand():
     md.tree_mask = None
     assert md.tree_mask is None
     assert dataclasses.replace(md, tree_mask=m).tree_mask is m
+
+
+@pytest.mark.parametrize("trees", ["0", "1"])
+def test_no_mask_beside_a_longer_chunk(monkeypatch, trees):
+    """A row's mask has 64 bits: metadata of longer chunks refuses masks, before
+    any layer runs."""
+    monkeypatch.setenv("GFX906_FA_TREES", trees)
+    step = _step(65, seqs=1)
+    cfg = types.SimpleNamespace(scheduler_config=types.SimpleNamespace(max_num_seqs=4, max_num_batched_tokens=400))
+    md = _builder(cfg).build(0, step)
+    with pytest.raises(RuntimeError, match="64 query tokens"):
+        md.tree_mask = torch.full((65,), -1, dtype=torch.int64)
+    assert md.tree_mask is None
+    assert _builder(cfg).build_for_cudagraph_capture(step).tree_mask is None
+    fields = {f.name: getattr(md, f.name) for f in dataclasses.fields(md) if f.name != "graph_masks"}
+    with pytest.raises(RuntimeError, match="64 query tokens"):
+        Gfx906FAMetadata(**{**fields, "tree_mask": torch.full((65,), -1, dtype=torch.int64)})

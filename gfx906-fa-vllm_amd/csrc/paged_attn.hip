@@ -1112,14 +1112,18 @@ __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void at
         d.upw = 0;
         d.nwg = dec_nwg(p, d.Uv, nseg);
         const int maxc = p.nwg / Hkv;  // pieces of all sequences, at most
-        if (nseg > 0 && nseg <= maxc && tot < (1 << 24)) {
+        if (SC != SC_NONE && p.whole) {
+            // one piece a segment, whatever its length: no merge follows (the
+            // host has checked that there is a workgroup for each)
+            lc = ln > 0 ? 1 : 0;
+            cincl = wave_incl_scan(lc);
+            d.upw = INT32_MAX;
+            d.nwg = nseg * Hkv;
+        } else if (nseg > 0 && nseg <= maxc && tot < (1 << 24)) {
             // the even share (in floats: one too few only costs a try), then
             // what stream-K would give each workgroup, and a little
             const float even = 16.0f * (float)tot / (float)maxc;
             int upw = max((int)ceilf(even), 16 * GFA_DEC_ALIGN_UNITS);
-            if constexpr (SC != SC_NONE) {
-                if (p.whole) upw = 1 << 20;  // (the host has checked nseg <= maxc)
-            }
             for (int t = 0; t < 2 && d.upw == 0; ++t) {
                 lc = ln > 0 ? pl_div(16 * ln + upw - 1, upw) : 0;
                 cincl = wave_incl_scan(lc);
@@ -3577,7 +3581,7 @@ struct Plan {
     size_t list_extra;  // bytes of the work list past 20 an item (see the allocation-free entry)
     size_t bytes;       // the regions a call needs; the tile images follow at `bytes`
     size_t img_bytes;   // room the tile images of the call's shape can take (capped)
-    int64_t max_seq_len;
+    int said_len;       // the caller's max_seq_len, 0 where it says nothing (scored calls)
     bool comb_short;    // contexts of at most GFA_COMB_FEW_KEYS keys (combine choice)
 };
 
@@ -3776,7 +3780,6 @@ Plan make_plan(int num_seqs, int num_tokens, int num_heads, int num_kv_heads, in
     pl.pf_rows = max_rows <= GFA_PF_KS2_MAX_ROWS ? PF_ROWS / 2 : PF_ROWS;
     plan_finish(pl, num_seqs, num_tokens, G, num_kv_heads, false, allow_split, max_seq_len, max_query_len);
     pl.comb_short = max_seq_len <= GFA_COMB_FEW_KEYS;
-    pl.max_seq_len = max_seq_len;
     return pl;
 }
 
@@ -3873,7 +3876,7 @@ hipError_t launch_all(const AttnParams &p0, const Plan &pl, char *ws, int num_se
             const bool wide = c.nrg == 3 || (c.nrg == 2 && c.rows_hi > 32);
             const int64_t most = (int64_t)num_seqs * num_kv_heads >= device_cus() ? 1024 : wide ? 128 : 384;
             const int wgs = c.nrg == 2 && !wide ? c.nwg * DEC_NW / dec_nw(2, false) : c.nwg;
-            pd.whole = num_seqs <= min(64, wgs / num_kv_heads) && pl.max_seq_len <= most;
+            pd.whole = num_seqs <= min(64, wgs / num_kv_heads) && pl.said_len > 0 && pl.said_len <= most;
             merge = !pd.whole;
         }
         // combine rows: a split segment has at most min(max_query_len * G, slot) rows
@@ -4240,6 +4243,7 @@ hipError_t paged_attention_impl(
     }
 
     if (scores) {
+        pl.said_len = max_seq_len;
         if (scores->cap > 0.0f) return launch_scored<SC_CAP>(p, pl, ws, q_dtype, out_dtype, max_query_len, stream);
         if (scores->slopes) return launch_scored<SC_BIAS>(p, pl, ws, q_dtype, out_dtype, max_query_len, stream);
         if (scores->tree) return launch_scored<SC_TREE>(p, pl, ws, q_dtype, out_dtype, max_query_len, stream);

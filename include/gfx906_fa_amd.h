@@ -474,7 +474,10 @@ hipError_t gfx906_fa_amd_paged_attention_padded(
  *                     64.
  *     soft_cap and tree_mask go together; alibi_slopes alone.  Without any of
  *     them the call is (5).  query fp16 or bf16, out of its type or fp32.
- *     Workspace and plan as (5).  A row that sees no key is 0.  With one of
+ *     Workspace and plan as (5), with max_seq_len choosing between segments in
+ *     one piece and split ones: lengths above it are right, but one workgroup
+ *     may then read a long segment alone (0 says nothing: split).
+ *     A row that sees no key is 0.  With one of
  *     them, K and V of keys that no row sees, or that some row does not see,
  *     may hold anything; a V block a row sees has to have a finite scale, and
  *     values within +-65504 where the row is of a prefill-shaped sequence

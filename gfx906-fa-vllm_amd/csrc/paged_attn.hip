@@ -172,8 +172,11 @@ struct AttnParams {
 constexpr int SC_NONE = 0, SC_TREE = 1, SC_CAP = 2, SC_BIAS = 3;
 
 // cap * tanh(s / cap) in log2 units, from x = 2 log2 e * s / cap: with t = 2^x,
-// tanh = 1 - 2 / (1 + t), exact at both ends (t = 0, inf) and within 1.2e-7 * cap
-// of it between: at the largest cap taken, 1024, a quarter of fp16's half step.
+// tanh = 1 - 2 / (1 + t), exact at both ends (t = 0, inf).  Between them v_exp and
+// v_rcp are within an ulp: 3 * 2^-23 with the rounding of 1 + t, and 2^-23 for the
+// cap's and the result's, 4.8e-7 * cap at most; measured over x in [-40, 40],
+// 2.5e-7.  At the largest cap taken, 1024, that moves a weight by 2.6e-4, about
+// half of fp16's half step.
 // less: subtracted from the result (a running max).
 __device__ __forceinline__ float capped(float x, float cap_log2e, float less) {
     return fmaf(-2.0f * cap_log2e, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x)), cap_log2e - less);
@@ -470,27 +473,6 @@ struct SubPageS {
     u32x4 kq[2], ks[2], vq[2], vs[2];
 };
 
-template <bool NT>
-__device__ __forceinline__ void load_subpage(SubPageS &sp, const uint8_t *kb, const uint8_t *vb,
-                                             const LaneOffsets &lo) {
-    const u32x4 *k0 = reinterpret_cast<const u32x4 *>(kb + lo.kq);
-    const u32x4 *ks = reinterpret_cast<const u32x4 *>(kb + lo.vs);  // (the offset of tokens 4g .. in either table)
-    const u32x4 *v0 = reinterpret_cast<const u32x4 *>(vb + lo.vq);
-    const u32x4 *vs = reinterpret_cast<const u32x4 *>(vb + lo.vs);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if constexpr (NT) {
-            sp.kq[i] = __builtin_nontemporal_load(k0 + 64 * i);
-            sp.vq[i] = __builtin_nontemporal_load(v0 + 64 * i);
-        } else {
-            sp.kq[i] = k0[64 * i];
-            sp.vq[i] = v0[64 * i];
-        }
-        sp.ks[i] = ks[i];
-        sp.vs[i] = vs[i];
-    }
-}
-
 // attend_subpage with the scored forms.  K's int8 values enter the MFMA as they
 // are, and the scores of its four blocks are scaled and added in fp32 (16
 // mixed-precision multiply-adds a row group, the count of packed products that
@@ -609,11 +591,11 @@ __device__ __forceinline__ void load_rows(const AttnParams &p, int h, int q0, in
 // and a sub-page's address is scalar arithmetic (no division per sub-page).
 // j0 / jstep: the wave takes sub-pages j0, j0 + jstep, ... of the range (the
 // waves of a workgroup interleave over one range).
-template <int NRG, bool NT, int DEPTH, int SC = SC_NONE>
+template <int NRG, bool NT, int DEPTH>
 __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams &p, int s, int h,
                                              int wb, int we, const half8_t (&qf)[NRG][4],
-                                             const int (&lim)[NRG], const ScoreRows<NRG, SC> &sr, int lane, int i16,
-                                             int g, int j0 = 0, int jstep = 1) {
+                                             const int (&lim)[NRG], int lane, int i16, int g,
+                                             int j0 = 0, int jstep = 1) {
     const int nall = (we - wb + 15) >> 4;
     const int nsub = nall > j0 ? (nall - j0 + jstep - 1) / jstep : 0;  // this wave's sub-pages
     if (nsub <= 0) return;
@@ -645,8 +627,7 @@ __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams
     const float c = p.scale_log2e;
     const LaneOffsets lo = lane_offsets(i16, g);
 
-    using SP = std::conditional_t<SC == SC_NONE, SubPage, SubPageS>;
-    auto fetch = [&](SP &sp, int j) {
+    auto fetch = [&](SubPage &sp, int j) {
         if (j < nsub) {
             if ((j >> 6) != chunk) {  // advance the page-id window (uniform)
                 chunk = j >> 6;
@@ -661,7 +642,7 @@ __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams
         }
     };
     // ring of DEPTH sub-page buffers: DEPTH-1 sub-pages in flight while one computes
-    SP buf[DEPTH];
+    SubPage buf[DEPTH];
 #pragma unroll
     for (int u = 0; u < DEPTH - 1; ++u) fetch(buf[u], u);
     for (int base = 0; base < nsub; base += DEPTH) {
@@ -671,9 +652,8 @@ __device__ __forceinline__ void stream_range(WaveAcc<NRG> &acc, const AttnParams
             if (j < nsub) {  // uniform
                 fetch(buf[(u + DEPTH - 1) % DEPTH], j + DEPTH - 1);
                 const int tok0 = wb + 16 * (j0 + jstep * j);
-                const bool mask = !(tok0 + 16 <= we && tok0 + 15 <= lim_min);
-                if constexpr (SC == SC_NONE) attend_subpage<NRG>(acc, buf[u], qf, tok0, we, lim, c, g, mask);
-                else attend_subpage_scored<NRG, SC>(acc, buf[u], qf, tok0, we, lim, sr, c, g, mask);
+                attend_subpage<NRG>(acc, buf[u], qf, tok0, we, lim, c, g,
+                                    !(tok0 + 16 <= we && tok0 + 15 <= lim_min));
             }
         }
     }
@@ -1301,9 +1281,9 @@ __attribute__((amdgpu_waves_per_eu(DecCfg<NRG>::wpe, DecCfg<NRG>::wpe))) void at
             stream_range_lds<NRG, DEC_RING, SC>(acc, p, s, h, 16 * a, min(16 * b, si.kv_lim), qf, lim, sr, lane, i16,
                                                 g, j0, jstep, reinterpret_cast<uint8_t *>(&sm_o[wv][0][0]));
         } else {
-            stream_range<NRG, GFA_DEC_NT != 0, DecCfg<NRG>::depth, SC>(acc, p, s, h, 16 * a,
-                                                                         min(16 * b, si.kv_lim), qf, lim, sr,
-                                                                         lane, i16, g, j0, jstep);
+            stream_range<NRG, GFA_DEC_NT != 0, DecCfg<NRG>::depth>(acc, p, s, h, 16 * a,
+                                                                     min(16 * b, si.kv_lim), qf, lim,
+                                                                     lane, i16, g, j0, jstep);
         }
         // ---- merge the chunk's waves' states in LDS ------------------------
         // in passes of 32 rows (row groups 2*ps, 2*ps + 1): a wave's LDS
@@ -2118,7 +2098,10 @@ __attribute__((amdgpu_waves_per_eu(3, 3))) void attn_prefill_kernel(AttnParams p
         KS == 2 ? lds + STAGES + w * PF_QBYTES + (lane & 31) * PF_KPITCH + 32 * (8 - QLDS) + 16 * hb
                 : lds + STAGES + w * QLDS * 1024 + 16 * lane;
     {
-        const float c = p.pf_qmul;  // a power of two: exact for fp16 / bf16 Q
+        // a power of two, exact for fp16 / bf16 Q; with a cap it goes down to
+        // 2^-8, where Q below 2^-6 is rounded to multiples of 2^-16 (half of one
+        // is fp16's half step at 2^-6: 2^-17 sum |k| times the scale in a score)
+        const float c = p.pf_qmul;
         const int64_t qrow = (int64_t)(q0 + j) * p.q_ts + (int64_t)hq * p.q_hs;  // (rows past nrows: row j = 0)
         uint8_t *const ql = KS == 2 ? lds + STAGES + w * PF_QBYTES
                                     : (w < 4 ? ldsk + PF_KBYTES : ldsv + PF_VBYTES) + (w & 3) * PF_QBYTES;

@@ -462,7 +462,9 @@ hipError_t gfx906_fa_amd_paged_attention_padded(
 
 /* (11) Scored paged attention: (5) with another score.  With s = scale * q.k
  *     soft_cap > 0:   cap * tanh(s / cap), cap at most 1024 and 1/32 to
- *                     32768 times the scale
+ *                     32768 times the scale (prefill-shaped sequences hold
+ *                     cap-scaled Q and K in fp16: with caps below the scale
+ *                     queries up to 8K and keys up to 5.6K stay finite)
  *     alibi_slopes:   s + slopes[head] * (key position - row position); fp32
  *                     [num_heads], row j at position seq_len - n_q + j (or
  *                     q_abs_offset + j)

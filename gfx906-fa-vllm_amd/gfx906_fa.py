@@ -614,7 +614,7 @@ MAX_TREE_NODES = 64
 MAX_SOFT_CAP = 1024.0  # the fp32 tanh's error grows with the cap
 
 
-_get_device = torch._C._cuda_getDevice
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _all_on(i: int, tensors, names: str) -> None:

@@ -99,3 +99,21 @@ def test_hidden_tokens_past_fp16(form, name, dt):
         b.key[int(r)] = (big * sign).to(b.key.dtype)
     _write(b)
     assert torch.equal(_call(b, form)[rows], want)
+
+
+@pytest.mark.parametrize("form", ["cap", "bias"])
+def test_seen_values_past_fp16(form):
+    """A value of 1e5 that a row does see: itself for decode rows, fp16's largest
+    where the row is of a prefill-shaped sequence."""
+    need_gpu()
+    announce(f"seen {form}")
+    for tokens, want in ((1, 1e5), (90, 65504.0)):
+        b = W.build_batch([tokens], [tokens], 8, 1, dtype="bf16", seed=3, device=DEV)
+        b.value.zero_()
+        b.value[0] = 1e5
+        _write(b)
+        out = _call(b, form)
+        want = min(want, float(b.value[0].max()))  # (bf16 holds 1e5 as 99840)
+        # the first row sees this key alone: Q8_0's scale, fp16, is off by 2^-11, p d_v by as much
+        assert ((out[0] - want).abs() <= 2.0 ** -10 * want).all()
+        assert torch.isfinite(out).all()

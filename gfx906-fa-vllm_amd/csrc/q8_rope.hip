@@ -400,7 +400,8 @@ __device__ __forceinline__ void load_cs_f32(const void *row, int col, float (&v)
 // 5.0 with 8; 8192 tokens: 68.4 us with 32, 66.2 with 16, 73.2 with 8).  16
 // against 8 rows, bf16, buffers out of cache: 1024 waves (16/16, 512 tokens) 7.8
 // and 6.8 us; 2048 (48/8, 512; 16/16, 1024) 6.6 and 7.8, 9.8 and 9.7; 4096 (48/8,
-// 1024) 9.3 and 11.8.
+// 1024) 9.3 and 11.8.  With each token's slot in a page of its own, as in a decode
+// step: 1024 waves (48/8, 256) 5.4 and 5.6, 2048 7.5 and 8.5, 4096 11.3 and 12.7.
 constexpr int NORM_ITERS = 4, NORM_FEW_ITERS = 2;
 constexpr int NORM_FEW_WAVES = 2048;
 

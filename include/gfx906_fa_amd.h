@@ -187,8 +187,8 @@ hipError_t gfx906_fa_amd_rope_cache_write_kv(
  *     q-head hq reads kv-head hq / (Hq/Hkv).  A row with no visible key is 0.
  *     Bytes behind a sequence's last key may hold anything, but decode-shaped
  *     sequences need finite V scales there (a zeroed or recycled page's are).
- *     Prefill-shaped ones hold V in fp16: values a row sees have to lie within
- *     +-65504.
+ *     Prefill-shaped ones hold V in fp16: a sequence's values have to lie
+ *     within +-65504.
  *     Numerics: dequantize-then-fp32 softmax (scores, max, sum and output
  *     accumulated in fp32; K int8 values enter the MFMA exactly and their
  *     scales are applied to the fp32 products; V scales are folded into P).

@@ -122,14 +122,15 @@ class _GraphMasks:
             return
         if masks is not None and masks.data_ptr() == self.buffer.data_ptr():
             return  # (the captured steps' own)
+        n = md.num_actual_tokens
+        if masks is not None:
+            if masks.dtype != torch.int64 or masks.dim() != 1 or masks.shape[0] < n:
+                raise RuntimeError("GFX906_FA: tree_mask must be int64 [num_tokens]")
+            if n > self.buffer.shape[0]:
+                raise RuntimeError(f"GFX906_FA: {n} tokens exceed max_num_batched_tokens ({self.buffer.shape[0]})")
         self.causal()
         if masks is None:
             return
-        n = md.num_actual_tokens
-        if masks.dtype != torch.int64 or masks.dim() != 1 or not n <= masks.shape[0]:
-            raise RuntimeError("GFX906_FA: tree_mask must be int64 [num_tokens]")
-        if n > self.buffer.shape[0]:
-            raise RuntimeError(f"GFX906_FA: {n} tokens exceed max_num_batched_tokens ({self.buffer.shape[0]})")
         self.buffer[:n].copy_(masks[:n])
         self._masks = True
 

@@ -84,6 +84,11 @@ def test_graphs_read_the_steps_masks(monkeypatch):
     for bad in (_masks(5).int(), _masks(5)[:-1], _masks(5)[None]):
         with pytest.raises(RuntimeError, match="int64"):
             b.build(0, _step(5)).tree_mask = bad
+    md = b.build(0, _step(5))
+    md.tree_mask = _masks(5)
+    with pytest.raises(RuntimeError, match="int64"):  # a refused mask changes nothing
+        md.tree_mask = _masks(5).int()
+    assert torch.equal(seen, _masks(5)) and torch.equal(md.tree_mask, _masks(5))
     with pytest.raises(RuntimeError, match="max_num_batched_tokens"):
         b.build(0, _step(30)).tree_mask = _masks(30)
     with pytest.raises(RuntimeError, match="max_num_batched_tokens"):
